@@ -1,0 +1,132 @@
+/* C-ABI of the serving operators around the fused attention, for sm_100a (B200): rotary positions (forward and gradient),
+ * appending new tokens' keys and values to a paged cache, attention of new tokens over that cache, and the handling of
+ * the cache's pages.
+ *
+ * Plain pointers and sizes only; every function returns a tx_dot_status code (b200_dot.h) and tx_paged_last_error()
+ * holds the text of this thread's last failure. Calls are asynchronous on `stream` (a cudaStream_t), allocate nothing on
+ * the device and keep nothing between calls: workspaces are the caller's, so calls on several streams, from several
+ * threads or in several CUDA graphs do not meet anywhere but in the per-device status word that tx_paged_check reads.
+ * There is no CPU path: without an sm_100 device every compute entry point returns TXD_ERR_NO_DEVICE.
+ */
+#ifndef B200_PAGED_H_
+#define B200_PAGED_H_
+
+#include <stdint.h>
+
+#include "b200_dot.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define TX_ROPE_MAX_PAIRS 128
+
+/* Rotary positions: pair i of the first `rotary_dim` columns of a head is turned by position * turns[i] / 2^64 of a full
+ * turn and multiplied by `magnitude`; the other columns pass unchanged. Pairs are columns (i, i + rotary_dim / 2), or
+ * (2 i, 2 i + 1) when interleaved. The products of a 64-bit position and the 64-bit fraction wrap at whole turns, so
+ * angles are as exact at position 2^31 as at position 1. */
+typedef struct tx_rope {
+  int32_t rotary_dim; /* even, 2 .. 256, at most the head dimension */
+  int32_t interleaved;
+  float magnitude;
+  int32_t reserved;
+  uint64_t turns[TX_ROPE_MAX_PAIRS];
+} tx_rope;
+
+/* One tensor [batch, heads, tokens, head_dim] that is turned; strides in elements, head_dim contiguous. `out` may be `in`
+ * (with the same strides); apart from that the two may not overlap. */
+typedef struct tx_rotary_part {
+  const void *in;
+  void *out;
+  int64_t in_stride[3];  /* batch, head, token */
+  int64_t out_stride[3]; /* batch, head, token */
+  int32_t heads;
+  int32_t reserved;
+} tx_rotary_part;
+
+typedef struct tx_rotary_problem {
+  int32_t batch, tokens, head_dim;
+  int32_t dtype;               /* TXD_F16, TXD_BF16 or TXD_F32 */
+  int32_t inverse;             /* 1: turn back; this is the gradient of the forward */
+  int32_t positions_64;        /* positions are int64 (1) or int32 (0) */
+  int64_t position_stride[2];  /* batch (0: shared), token; in elements */
+  int32_t parts;               /* 1 or 2 */
+  int32_t reserved;
+  tx_rotary_part part[2];
+} tx_rotary_problem;
+
+TXD_API int tx_rotary(const tx_rope *rope, const tx_rotary_problem *problem, const void *positions, void *stream);
+
+/* A paged cache as attention and append see it. Position p of sequence b lives in page table[b * table_stride + p / page_size],
+ * slot p % page_size. k and v: [num_pages, page_size, kv_heads, head_dim] with head_dim contiguous and the other strides
+ * free (multiples of 16 bytes). `kv_lens[b]` counts the cached tokens with the new ones; `cu_q` [batch + 1] holds where
+ * each sequence's new tokens start among all new tokens (NULL: one new token for each sequence). Sequence b's new tokens
+ * are its last ones: token j of q_len has position kv_lens[b] - q_len + j. Table entries that no used position needs are
+ * not read; an entry outside [0, num_pages) that is needed reads as zeros, is not written, and is reported by
+ * tx_paged_check. */
+typedef struct tx_paged_view {
+  void *k, *v;
+  int64_t k_stride[3], v_stride[3]; /* page, slot, head; in elements */
+  const int32_t *table;
+  int64_t table_stride;
+  const int32_t *kv_lens;
+  const int32_t *cu_q;
+  int32_t batch, table_width, num_pages, page_size; /* page_size: 16, 32, 64, 128 or 256 */
+  int32_t kv_heads, head_dim, dtype, reserved;      /* TXD_F16 or TXD_BF16 */
+} tx_paged_view;
+
+/* Writes the new tokens' k (turned, when `rope` is given) and v to their places in the cache and the turned q to q_out
+ * (which may be q). q, k, v, q_out: [tokens, heads, head_dim], strides in elements (token, head). `q` may be NULL
+ * (q_heads 0). Tokens behind the last sequence are left alone. */
+typedef struct tx_append_problem {
+  const void *q, *k, *v;
+  void *q_out;
+  int64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2];
+  int32_t tokens, q_heads;
+} tx_append_problem;
+
+TXD_API int tx_paged_append(const tx_paged_view *cache, const tx_rope *rope, const tx_append_problem *problem, void *stream);
+
+/* The pages of a cache and who holds them. k and v: [layers, num_pages, page_bytes]; table: [rows, width], -1 where a row
+ * has no page; lens[row]: its tokens; refs[page]: in how many table cells it stands (0: free). All on the device, changed
+ * in stream order, without the host. What is wrong with a call is found on the device and reported by tx_paged_check: a
+ * row outside the table is passed over by free and fork; a reserve with such a row, a row listed twice, a negative count,
+ * no room in a row or too few free pages does nothing at all.
+ * `workspace`: tx_pages_workspace(state, n) bytes, 16-byte aligned, of the caller; free again when the call has run. */
+typedef struct tx_pages_state {
+  void *k, *v;
+  int64_t page_bytes; /* of one layer's k (or v), a multiple of 16 */
+  int32_t *table, *lens, *refs;
+  int32_t layers, num_pages, page_size, rows, width, reserved;
+} tx_pages_state;
+
+#define TX_PAGES_MAX_LIST 4096 /* rows in one reserve */
+
+TXD_API int64_t tx_pages_workspace(const tx_pages_state *state, int32_t n);
+/* Gives the pages of the listed rows back and empties the rows (a row may be listed twice). */
+TXD_API int tx_pages_free(const tx_pages_state *state, const int32_t *rows, int32_t n, void *stream);
+/* Row dst[i] becomes what row src[i] was before the call, sharing its pages; what dst[i] held is given back. Sources may be
+ * destinations too (a reordering); where a destination is listed twice the last one holds. */
+TXD_API int tx_pages_fork(const tx_pages_state *state, const int32_t *dst, const int32_t *src, int32_t n, void *workspace,
+                          void *stream);
+/* Makes room for counts[i] more tokens in each listed row and adds them to its length: new pages are the lowest free ones,
+ * in list order; a partly filled last page that other rows share is copied first (of the listed rows that share it alone,
+ * the last keeps it). */
+TXD_API int tx_pages_reserve(const tx_pages_state *state, const int32_t *rows, const int32_t *counts, int32_t n,
+                             void *workspace, void *stream);
+/* Moves pages so that the used ones are the lowest: with U pages in use, those at U and above go to the free ones below, in
+ * order, and the table follows. */
+TXD_API int tx_pages_compact(const tx_pages_state *state, void *workspace, void *stream);
+/* Copies pages src[i] to dst[i] in every layer (host lists). No page may be a destination twice, or source and destination. */
+TXD_API int tx_pages_copy(const tx_pages_state *state, const int32_t *src, const int32_t *dst, int32_t n, void *stream);
+
+/* Synchronises `stream` and reports (and clears) what kernels of this header found on the device since the last check. */
+TXD_API int tx_paged_check(void *stream);
+
+TXD_API uint64_t tx_paged_kernel_launches(void);
+TXD_API const char *tx_paged_last_error(void);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* B200_PAGED_H_ */

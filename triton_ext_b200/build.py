@@ -7,7 +7,7 @@ infra/pass/CMakeLists.txt:3-14):
     lib/libTritonExtPassInfra.so   registry + loop IR + pass manager
     lib/libloop_split.so           pass extension   (pass/LoopSplit)
     lib/libdot_tile_select.so      pass extension   (pass/DotTileSelect)
-    lib/libb200_dot.so             backend extension: sm_100a kernels (tt.dot GEMM, fused attention forward)
+    lib/libb200_dot.so             backend extension: sm_100a kernels (tt.dot GEMM, fused attention, paged cache)
                                    + launch C-ABI + lowering pass
 
 Each extension is named by its `triton-ext.conf` and is skipped when TRITON_EXT_NAMES is set and
@@ -33,7 +33,8 @@ EXTENSIONS = [
     ("pass/LoopSplit", "LoopBisectPass", ["LoopSplitPass.cpp", "LoopSplitText.cpp"], False),
     ("pass/DotTileSelect", "DotTileSelectPass", ["DotTileSelectPass.cpp"], False),
     ("backend/B200Dot", "B200DotLoweringPass", ["b200_dot.cu", "b200_dot_static.cu", "B200DotLowering.cpp",
-                                                   "../B200Attention/b200_attention.cu"], True),
+                                                   "../B200Attention/b200_attention.cu",
+                                                   "../B200Paged/b200_paged.cu"], True),
 ]
 
 CXXFLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall"]
@@ -84,16 +85,17 @@ def build_all(force: bool = False, verbose: bool = False, ptxas_verbose: bool = 
         meta = conf.read_conf(d)
         out = os.path.join(LIB, f"lib{meta.name}.so")
         deps = (common_deps + _all_sources(d) + _all_sources(os.path.join(CSRC, "backend", "B200Dot")) +
-                _all_sources(os.path.join(CSRC, "backend", "B200Attention")))
+                _all_sources(os.path.join(CSRC, "backend", "B200Attention")) +
+                _all_sources(os.path.join(CSRC, "backend", "B200Paged")))
         if force or _stale(out, deps):
             defs = [f"-DTRITON_EXT_NAME={meta.name}", f"-DTRITON_EXT_CLASS={cls}"]
             incs = ["-I", INCLUDE, "-I", os.path.join(CSRC, "infra"), "-I", os.path.join(CSRC, "backend", "B200Dot"),
-                    "-I", os.path.join(CSRC, "backend", "B200Attention")]
+                    "-I", os.path.join(CSRC, "backend", "B200Attention"), "-I", os.path.join(CSRC, "backend", "B200Paged")]
             link = ["-L", LIB, "-lTritonExtPassInfra"]
             srcs = [os.path.join(d, s) for s in sources]
             if cuda:
                 nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
-                cmd = [nvcc, *NVCC_ARCH, "-O3", "-std=c++17", "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden",
+                cmd = [nvcc, *NVCC_ARCH, "--threads", "0", "-O3", "-std=c++17", "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden",
                        *defs, *incs, *srcs, *link, "-Xlinker", "-rpath=$ORIGIN", "-o", out]
                 if ptxas_verbose:
                     cmd[1:1] = ["-Xptxas", "-v"]

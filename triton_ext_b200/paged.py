@@ -1,0 +1,255 @@
+"""A cache of keys and values in pages, and what a serving step does with it (include/b200_paged.h):
+
+  append            the new tokens' k (turned by their positions) and v into their pages, and the turned q
+  PagedCache        who holds which page, on the device: reserve, fork, free, compact, copy_pages
+
+A step is `cache.reserve(rows, counts)`, then for every layer `append`. Nothing in a step
+synchronises, reads the device or depends on the host knowing a length, so a step can be captured in a CUDA graph and
+replayed while the sequences grow. What kernels find wrong (a bad page, no free pages) is reported by `check`.
+
+torch is used for device memory and streams only. There is no fallback: if the shared library is missing or no B200 is
+present the calls raise.
+"""
+from __future__ import annotations
+
+import ctypes
+import struct
+from typing import Optional, Sequence
+
+import torch
+
+from . import backend as B
+from .rotary import Rope, _on, check  # noqa: F401  (check: part of this module's interface)
+
+_DTYPES = {torch.float16: B.TXD_F16, torch.bfloat16: B.TXD_BF16}
+MAX_LIST = 4096  # rows in one reserve
+
+_lib_cache = None
+
+
+def _lib() -> ctypes.CDLL:
+    global _lib_cache
+    if _lib_cache is None:
+        lib = B.load_library()
+        vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+        for name, args, res in (
+                ("tx_paged_append", [vp, vp, vp, vp], ctypes.c_int),
+                ("tx_pages_workspace", [vp, i32], i64),
+                ("tx_pages_free", [vp, vp, i32, vp], ctypes.c_int),
+                ("tx_pages_fork", [vp, vp, vp, i32, vp, vp], ctypes.c_int),
+                ("tx_pages_reserve", [vp, vp, vp, i32, vp, vp], ctypes.c_int),
+                ("tx_pages_compact", [vp, vp, vp], ctypes.c_int),
+                ("tx_pages_copy", [vp, vp, vp, i32, vp], ctypes.c_int)):
+            f = getattr(lib, name)
+            f.argtypes, f.restype = args, res
+        lib.tx_paged_last_error.restype = ctypes.c_char_p
+        lib.tx_paged_kernel_launches.restype = ctypes.c_uint64
+        _lib_cache = lib
+    return _lib_cache
+
+
+def _raise(lib, rc: int):
+    raise B.DotError(rc, lib.tx_paged_last_error().decode())
+
+
+def _invalid(text: str):
+    raise B.DotError(B.TXD_ERR_INVALID, text)
+
+
+def kernel_launches() -> int:
+    return int(_lib().tx_paged_kernel_launches())
+
+
+_VIEW = struct.Struct("2P6qPq2P8i")
+_APPEND = struct.Struct("4P8q2i")
+_STATE = struct.Struct("2Pq3P6i")
+
+
+def _view(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+          cu_q: Optional[torch.Tensor], device: torch.device) -> bytes:
+    shape, dtype = k_pages.shape, _DTYPES.get(k_pages.dtype)
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != k_pages.dtype:
+        _invalid("k_pages and v_pages must be [pages, page_size, kv_heads, head_dim] of one shape and type")
+    if dtype is None:
+        raise B.DotError(B.TXD_ERR_UNSUPPORTED, f"cache dtype {k_pages.dtype}: f16 and bf16 are built")
+    if not (k_pages.device == v_pages.device == page_table.device == kv_lens.device == device):
+        _invalid("the cache, page_table and kv_lens must be on the device of the new tokens")
+    ks, vs, ts = k_pages.stride(), v_pages.stride(), page_table.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        _invalid("head_dim must be the contiguous dimension of k_pages and v_pages")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or (ts[1] != 1 and page_table.shape[1] > 1):
+        _invalid("page_table must be int32 [batch, pages of a sequence] with unit column stride")
+    batch, width = page_table.shape
+    if kv_lens.dtype != torch.int32 or kv_lens.dim() != 1 or kv_lens.shape[0] != batch or (batch > 1 and kv_lens.stride(0) != 1):
+        _invalid(f"kv_lens must be a contiguous int32 vector of {batch} lengths")
+    if cu_q is not None and (cu_q.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] != batch + 1 or
+                             (batch > 0 and cu_q.stride(0) != 1) or cu_q.device != device):
+        _invalid(f"cu_q must be a contiguous int32 vector of {batch + 1} offsets on the device of the new tokens")
+    return _VIEW.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], page_table.data_ptr(),
+                      ts[0], kv_lens.data_ptr(), cu_q.data_ptr() if cu_q is not None else 0, batch, width, shape[0], shape[1],
+                      shape[2], shape[3], dtype, 0)
+
+
+def _token_strides(x: torch.Tensor, name: str, tokens: int, head_dim: int, like: torch.Tensor) -> tuple[int, int]:
+    if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != head_dim or x.dtype != like.dtype or x.device != like.device:
+        _invalid(f"{name} must be [tokens, heads, head_dim] = [{tokens}, *, {head_dim}] of the cache's type and device")
+    s = x.stride()
+    if s[2] != 1 and head_dim > 1:
+        _invalid(f"head_dim must be the contiguous dimension of {name}")
+    return s[0], s[1]
+
+
+def _not_cuda(q: torch.Tensor):
+    raise B.DotError(B.TXD_ERR_NO_DEVICE, f"CUDA tensors are wanted, got {q.device}: there is no CPU path")
+
+
+def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+           page_table: torch.Tensor, kv_lens: torch.Tensor, *, rope: Optional[Rope] = None, cu_q: Optional[torch.Tensor] = None,
+           out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Write the new tokens' k and v to their places in the cache and return q, q and k turned by their positions if a `rope`
+    is given. One launch on the current CUDA stream.
+
+    q, k, v: [tokens, heads, head_dim], any strides with head_dim contiguous (parts of one projection's output, say); q may
+    be None. k_pages, v_pages: [pages, page_size, kv_heads, head_dim]. page_table: int32 [batch, width]. kv_lens: int32
+    [batch], the sequences' lengths WITH the new tokens. cu_q: int32 [batch + 1], where each sequence's new tokens start
+    (None: one token for each sequence, in order). Sequence b's new tokens take its last positions. out: where the turned q
+    goes (q itself is allowed). Tokens behind cu_q[-1] are left alone: their rows of `out` are not written."""
+    lib = _lib()
+    if not k.is_cuda:
+        _not_cuda(k)
+    view = _view(k_pages, v_pages, page_table, kv_lens, cu_q, k.device)
+    tokens, heads, d = k.shape if k.dim() == 3 else _invalid("k must be [tokens, kv_heads, head_dim]")
+    if heads != k_pages.shape[2] or v.shape != k.shape or d != k_pages.shape[3]:
+        _invalid("k and v must be [tokens, kv_heads, head_dim] with the cache's heads and head_dim")
+    if cu_q is None and tokens != page_table.shape[0]:
+        _invalid(f"without cu_q there is one new token for each of the {page_table.shape[0]} sequences, got {tokens}")
+    ks, vs = _token_strides(k, "k", tokens, d, k_pages), _token_strides(v, "v", tokens, d, k_pages)
+    q_ptr, o_ptr, q_heads, qs, os_ = 0, 0, 0, (0, 0), (0, 0)
+    if q is not None:
+        qs, q_heads = _token_strides(q, "q", tokens, d, k_pages), q.shape[1]
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or (tokens > 1 and out.stride(0) == 0) or (q_heads > 1 and out.stride(1) == 0):
+            _invalid("out must have the shape of q and not be an expanded tensor")
+        os_ = _token_strides(out, "out", tokens, d, k_pages)
+        q_ptr, o_ptr = q.data_ptr(), out.data_ptr()
+    elif out is not None:
+        _invalid("out is for the turned q: there is none")
+    if rope is not None and rope.rotary_dim > d:
+        _invalid(f"rotary_dim {rope.rotary_dim} exceeds head_dim {d}")
+    problem = _APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, *qs, *ks, *vs, *os_, tokens, q_heads)
+    with _on(k.device) as stream:
+        rc = lib.tx_paged_append(view, rope._packed if rope is not None else None, problem, stream)
+    if rc:
+        _raise(lib, rc)
+    return out
+
+
+class PagedCache:
+    """A cache of `layers` pools of pages and the device-side record of who holds them.
+
+    k, v    [layers, pages, page_size, kv_heads, head_dim], contiguous, f16 or bf16; `k[layer]` is what `append` and
+            `paged_attention` take
+    table   int32 [rows, width]: the pages of each row (a sequence), -1 where there is none
+    lens    int32 [rows]: its tokens
+    refs    int32 [pages]: in how many table cells a page stands; 0: free
+
+    The operations take rows as int32 CUDA vectors, run in stream order and never synchronise; a row outside the table is
+    passed over (by `reserve`: nothing is done at all) and reported by `check`."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor):
+        if k.dim() != 5 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _DTYPES:
+            _invalid("k and v must be [layers, pages, page_size, kv_heads, head_dim] of one shape and type, f16 or bf16")
+        for name, t, dims in (("table", table, 2), ("lens", lens, 1), ("refs", refs, 1)):
+            if t.dtype != torch.int32 or t.dim() != dims:
+                _invalid(f"{name} must be int32 with {dims} dimension(s)")
+        if lens.shape[0] != table.shape[0] or refs.shape[0] != k.shape[1]:
+            _invalid("lens must have one entry for each row of table, refs one for each page")
+        for name, t in (("k", k), ("v", v), ("table", table), ("lens", lens), ("refs", refs)):
+            if not t.is_contiguous():
+                _invalid(f"{name} must be contiguous")
+            if t.device != k.device:
+                _invalid("k, v, table, lens and refs must be on one device")
+        self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
+        layers, pages, page_size, heads, d = k.shape
+        self.page_size = page_size
+        self._state = _STATE.pack(k.data_ptr(), v.data_ptr(), page_size * heads * d * k.element_size(), table.data_ptr(),
+                                  lens.data_ptr(), refs.data_ptr(), layers, pages, page_size, table.shape[0], table.shape[1], 0)
+
+    @classmethod
+    def create(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, *, rows: int, width: int, layers: int = 1,
+               dtype: torch.dtype = torch.bfloat16, device="cuda") -> "PagedCache":
+        """An empty cache; the pools are not initialised."""
+        k, v = (torch.empty((layers, pages, page_size, kv_heads, head_dim), dtype=dtype, device=device) for _ in range(2))
+        table = torch.full((rows, width), -1, dtype=torch.int32, device=k.device)
+        return cls(k, v, table, torch.zeros(rows, dtype=torch.int32, device=k.device),
+                   torch.zeros(pages, dtype=torch.int32, device=k.device))
+
+    def _list(self, x: torch.Tensor, name: str, n: Optional[int] = None) -> torch.Tensor:
+        if not self.k.is_cuda:
+            _not_cuda(self.k)
+        if x.dtype != torch.int32 or x.dim() != 1 or x.device != self.k.device or (n is not None and x.shape[0] != n):
+            _invalid(f"{name} must be an int32 vector{f' of {n}' if n is not None else ''} on the device of the cache")
+        return x if x.is_contiguous() else x.contiguous()
+
+    def _workspace(self, lib, n: int) -> torch.Tensor:
+        return torch.empty(lib.tx_pages_workspace(self._state, n), dtype=torch.uint8, device=self.k.device)
+
+    def free(self, rows: torch.Tensor) -> None:
+        """Give the pages of the listed rows back (those that no other row holds become free) and empty the rows."""
+        lib, rows = _lib(), self._list(rows, "rows")
+        with _on(self.k.device) as stream:
+            rc = lib.tx_pages_free(self._state, rows.data_ptr(), rows.shape[0], stream)
+        if rc:
+            _raise(lib, rc)
+
+    def fork(self, dst: torch.Tensor, src: torch.Tensor) -> None:
+        """Row dst[i] becomes what row src[i] was before the call, sharing its pages. Rows may be both (the reordering of a
+        beam search); what a destination held is given back; of a destination listed twice the last one holds."""
+        lib, dst = _lib(), self._list(dst, "dst")
+        src = self._list(src, "src", dst.shape[0])
+        with _on(self.k.device) as stream:
+            ws = self._workspace(lib, dst.shape[0])
+            rc = lib.tx_pages_fork(self._state, dst.data_ptr(), src.data_ptr(), dst.shape[0], ws.data_ptr(), stream)
+        if rc:
+            _raise(lib, rc)
+
+    def reserve(self, rows: torch.Tensor, counts: torch.Tensor) -> None:
+        """Make room for counts[i] more tokens in row rows[i] and add them to its length, before they are appended. New pages
+        are the lowest free ones in list order. A partly filled last page that other rows share is copied first (all layers);
+        of the listed rows that alone share one, the last keeps it."""
+        lib, rows = _lib(), self._list(rows, "rows")
+        counts = self._list(counts, "counts", rows.shape[0])
+        with _on(self.k.device) as stream:
+            ws = self._workspace(lib, rows.shape[0])
+            rc = lib.tx_pages_reserve(self._state, rows.data_ptr(), counts.data_ptr(), rows.shape[0], ws.data_ptr(), stream)
+        if rc:
+            _raise(lib, rc)
+
+    def compact(self) -> None:
+        """Move pages (all layers) so that the used ones are the lowest, the fewest that do it; the table follows."""
+        lib = _lib()
+        if not self.k.is_cuda:
+            _not_cuda(self.k)
+        with _on(self.k.device) as stream:
+            ws = self._workspace(lib, 0)
+            rc = lib.tx_pages_compact(self._state, ws.data_ptr(), stream)
+        if rc:
+            _raise(lib, rc)
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Copy the contents of pages src[i] to dst[i] in every layer. Host lists; no page may be a destination twice, or
+        source and destination."""
+        lib, n = _lib(), len(src)
+        if not self.k.is_cuda:
+            _not_cuda(self.k)
+        if len(dst) != n:
+            _invalid("src and dst must be of one length")
+        pages = self.k.shape[1]
+        for x in (*src, *dst):
+            if not 0 <= int(x) < pages:
+                _invalid(f"page {x} is outside the {pages} pages")
+        with _on(self.k.device) as stream:
+            rc = lib.tx_pages_copy(self._state, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n, stream)
+        if rc:
+            _raise(lib, rc)
