@@ -87,6 +87,28 @@ typedef struct tx_append_problem {
 
 TXD_API int tx_paged_append(const tx_paged_view *cache, const tx_rope *rope, const tx_append_problem *problem, void *stream);
 
+/* Attention of the new tokens over their sequences' cached keys and values (which include their own: append first).
+ * Query head h reads key head h / (q_heads / kv_heads). With `causal` new token j sees the keys at positions up to its own,
+ * kv_lens[b] - q_len + j, and with `window` > 0 only the last `window` of them; without `causal` it sees all kv_lens[b].
+ * A row that sees no key gives zeros and m = -inf. What the cache holds at positions that no row of a sequence sees never
+ * matters (it may be NaN); keys and values that some row sees have to be finite.
+ * `m` (may be NULL): [tokens, q_heads] fp32, running max + log2(sum) in base 2 as tx_attn_fwd returns it. Rows behind the
+ * last sequence are left alone. `max_q` is the caller's bound on the new tokens of one sequence: it decides between the
+ * kernels for few and for many rows, not what is computed. Results are the same from run to run, and do not depend on the
+ * other sequences of the batch by more than the rounding of a different split. */
+typedef struct tx_paged_attn_problem {
+  const void *q; /* [tokens, q_heads, head_dim], strides in elements (token, head), multiples of 16 bytes */
+  void *out;     /* the same shape and type */
+  float *m;
+  int64_t q_stride[2], out_stride[2];
+  int32_t tokens, q_heads, max_q, causal, window;
+  float sm_scale;
+} tx_paged_attn_problem;
+
+TXD_API int64_t tx_paged_attention_workspace(const tx_paged_view *cache, const tx_paged_attn_problem *problem);
+TXD_API int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_problem *problem, void *workspace,
+                               int64_t workspace_bytes, void *stream);
+
 /* The pages of a cache and who holds them. k and v: [layers, num_pages, page_bytes]; table: [rows, width], -1 where a row
  * has no page; lens[row]: its tokens; refs[page]: in how many table cells it stands (0: free). All on the device, changed
  * in stream order, without the host. What is wrong with a call is found on the device and reported by tx_paged_check: a

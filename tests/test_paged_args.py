@@ -156,6 +156,7 @@ def test_cpu_tensors_are_refused_not_computed(built_libs):
     c = Built()
     x = torch.zeros(3, 2, 64, dtype=bf16)
     assert status_of(lambda: P.append(None, x, x, c.k, c.v, c.table, c.lens))[0] == B.TXD_ERR_NO_DEVICE
+    assert status_of(lambda: P.paged_attention(x, c.k, c.v, c.table, c.lens, 0.1))[0] == B.TXD_ERR_NO_DEVICE
     q = torch.zeros(1, 2, 3, 64, dtype=bf16)
     assert status_of(lambda: R.rotary_forward(q, None, torch.arange(3), R.Rope(64)))[0] == B.TXD_ERR_NO_DEVICE
     cache = P.PagedCache.create(4, 16, 2, 64, rows=3, width=2, device="cpu")

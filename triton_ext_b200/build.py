@@ -34,7 +34,8 @@ EXTENSIONS = [
     ("pass/DotTileSelect", "DotTileSelectPass", ["DotTileSelectPass.cpp"], False),
     ("backend/B200Dot", "B200DotLoweringPass", ["b200_dot.cu", "b200_dot_static.cu", "B200DotLowering.cpp",
                                                    "../B200Attention/b200_attention.cu",
-                                                   "../B200Paged/b200_paged.cu"], True),
+                                                   "../B200Paged/b200_paged.cu",
+                                                   "../B200Paged/b200_paged_attention.cu"], True),
 ]
 
 CXXFLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall"]

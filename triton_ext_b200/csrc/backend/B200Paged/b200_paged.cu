@@ -51,7 +51,7 @@ int device_ready(uint32_t **status) {
   return TXD_OK;
 }
 
-int check_view(const tx_paged_view *c) {
+int check_view(const tx_paged_view *c, tx_paged_view *out) {
   if (!c) return fail(TXD_ERR_INVALID, "null cache");
   if (c->dtype != TXD_F16 && c->dtype != TXD_BF16) return fail(TXD_ERR_UNSUPPORTED, "cache dtype must be f16 or bf16");
   if (c->batch < 0 || c->table_width < 0 || c->num_pages < 1 || c->kv_heads < 1)
@@ -63,6 +63,12 @@ int check_view(const tx_paged_view *c) {
   if (!c->k || !c->v) return fail(TXD_ERR_INVALID, "null cache pointer");
   if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
     return fail(TXD_ERR_INVALID, "cache pointers must be 16-byte aligned");
+  // a stride over one element says nothing: give it a value that every use can take
+  *out = *c;
+  const int32_t extent[3] = {c->num_pages, c->page_size, c->kv_heads};
+  for (int i = 0; i < 3; ++i)
+    if (extent[i] == 1) out->k_stride[i] = out->v_stride[i] = c->head_dim;
+  c = out;
   for (int i = 0; i < 3; ++i)
     if (c->k_stride[i] < 0 || c->v_stride[i] < 0 || c->k_stride[i] % 8 || c->v_stride[i] % 8)
       return fail(TXD_ERR_UNSUPPORTED, "cache strides must be non-negative multiples of 16 bytes");
@@ -145,11 +151,15 @@ int launch_rotary(RotaryParams &prm, const int *heads, int head_dim, int dtype, 
   return launch_rotary_t<__half>(prm, w.v, stream);
 }
 
+}  // namespace
+
 int shift_of(int page_size) {
   int s = 0;
   while ((1 << s) < page_size) ++s;
   return s;
 }
+
+namespace {
 
 int check_pages(const tx_pages_state *st) {
   if (!st) return fail(TXD_ERR_INVALID, "null state");
@@ -255,9 +265,11 @@ int tx_rotary(const tx_rope *rope, const tx_rotary_problem *pr, const void *posi
   return launch_rotary(prm, heads, pr->head_dim, pr->dtype, static_cast<cudaStream_t>(stream));
 }
 
-int tx_paged_append(const tx_paged_view *c, const tx_rope *rope, const tx_append_problem *pr, void *stream) {
-  int rc = check_view(c);
+int tx_paged_append(const tx_paged_view *cache, const tx_rope *rope, const tx_append_problem *pr, void *stream) {
+  tx_paged_view view;
+  int rc = check_view(cache, &view);
   if (rc) return rc;
+  const tx_paged_view *c = &view;
   if (!pr) return fail(TXD_ERR_INVALID, "null problem");
   if (pr->tokens < 0 || pr->q_heads < 0) return fail(TXD_ERR_INVALID, "tokens and q_heads must be >= 0");
   if (rope && (rc = check_rope(rope, c->head_dim))) return rc;

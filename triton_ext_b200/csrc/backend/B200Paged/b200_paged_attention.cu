@@ -1,0 +1,286 @@
+// Host side of paged attention (include/b200_paged.h): argument checks, the choice of kernel, TMA descriptors, launches.
+// There is no CPU path here: without an sm_100 device every compute entry point fails.
+#include <atomic>
+#include <climits>
+#include <cstdlib>
+#include <mutex>
+
+#include "paged_row_kernel.cuh"
+
+namespace txp {
+namespace {
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// One pool as {64 columns, slots, column groups, heads, pages}; a box is `box_rows` slots of one page and head, with all
+// column groups. Columns past head_dim (16 and 32) are out of bounds and arrive as zeros.
+int encode_pool(CUtensorMap *map, const void *ptr, const tx_paged_view &c, const int64_t *stride, int box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fail(TXD_ERR_NO_DEVICE, "cuTensorMapEncodeTiled is not available from the CUDA driver");
+  const int groups = c.head_dim > 64 ? c.head_dim / 64 : 1;
+  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(c.head_dim < 64 ? c.head_dim : 64), static_cast<cuuint64_t>(c.page_size),
+                              static_cast<cuuint64_t>(groups), static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.num_pages)};
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(stride[1]) * 2, 128, static_cast<cuuint64_t>(stride[2]) * 2,
+                                 static_cast<cuuint64_t>(stride[0]) * 2};
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(groups), 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(map, c.dtype == TXD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                         const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TXD_ERR_CUDA, "cuTensorMapEncodeTiled (pool) failed with code %d", static_cast<int>(r));
+  return TXD_OK;
+}
+
+struct RowShape {  // rows a CTA attends with, and CTAs per SM
+  int mt, ks, per_sm;
+};
+
+// Which kernel takes a call: a function of the group, the bound on a sequence's new tokens and the head dimension.
+RowShape row_shape(int kernel_d, int group, int max_q) {
+  const long long rows = static_cast<long long>(group) * (max_q > 0 ? max_q : 1);
+  if (rows <= 16) return {1, 4, kernel_d == 256 ? 1 : 2};
+  if (rows <= 32) return {2, 4, 1};
+  return {4, 2, 1};
+}
+
+int sm_count() {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return 148;  // no device: only sizes are asked for
+  }
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (!n) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    cached[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+struct Plan {
+  tx_paged_view view;
+  int kernel_d, group, rows, ctas;
+  RowShape shape;
+  size_t borders_bytes, part_bytes, ml_bytes;
+  int64_t bytes() const { return static_cast<int64_t>(borders_bytes + part_bytes + ml_bytes); }
+};
+
+int make_plan(const tx_paged_view *cache, const tx_paged_attn_problem *pr, Plan *plan) {
+  int rc = check_view(cache, &plan->view);
+  if (rc) return rc;
+  if (!pr) return fail(TXD_ERR_INVALID, "null problem");
+  const tx_paged_view &c = plan->view;
+  if (pr->tokens < 0 || pr->q_heads < 1) return fail(TXD_ERR_INVALID, "tokens must be >= 0 and q_heads >= 1");
+  if (pr->q_heads % c.kv_heads) return fail(TXD_ERR_INVALID, "q_heads %d is not a multiple of kv_heads %d", pr->q_heads, c.kv_heads);
+  plan->group = pr->q_heads / c.kv_heads;
+  if (plan->group > 64) return fail(TXD_ERR_UNSUPPORTED, "%d query heads to a key head: at most 64 are built", plan->group);
+  if (pr->tokens > 0 && pr->max_q < 1) return fail(TXD_ERR_INVALID, "max_q must be >= 1");
+  if (pr->window < 0 || (pr->window > 0 && !pr->causal)) return fail(TXD_ERR_INVALID, "a window is >= 0 and goes with causal");
+  if (!(pr->sm_scale > 0.f) || pr->sm_scale > 1e30f) return fail(TXD_ERR_INVALID, "sm_scale must be positive and finite");
+  if (static_cast<long long>(c.table_width) * c.page_size > (1ll << 30)) return fail(TXD_ERR_UNSUPPORTED, "a row of the page table holds more than 2^30 tokens");
+  if (c.cu_q == nullptr && pr->tokens != c.batch) return fail(TXD_ERR_INVALID, "without cu_q there is one new token for each of the %d sequences", c.batch);
+  plan->kernel_d = c.head_dim <= 64 ? 64 : c.head_dim;
+  int max_q = pr->max_q;
+  if (max_q > pr->tokens) max_q = pr->tokens;
+  plan->shape = row_shape(plan->kernel_d, plan->group, max_q);
+  plan->rows = plan->shape.mt * 16;
+  plan->ctas = sm_count() * plan->shape.per_sm;
+  plan->borders_bytes = (static_cast<size_t>(plan->ctas) * 16 + 255) / 256 * 256;
+  const size_t rows = static_cast<size_t>(plan->ctas) * 2 * plan->rows;
+  plan->part_bytes = rows * plan->kernel_d * 4;
+  plan->ml_bytes = rows * 8;
+  return TXD_OK;
+}
+
+// The programmatic attribute lets a kernel be scheduled while its predecessor drains; it waits for it before it touches
+// memory (griddepcontrol.wait).
+template <typename P>
+cudaError_t launch(void (*kernel)(P), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const P &p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// The kernel's shared-memory limit is raised once per device.
+template <typename P>
+cudaError_t allow_smem(void (*kernel)(P), int bytes, std::atomic<uint64_t> *done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (done->load(std::memory_order_acquire) >> dev & 1) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done->fetch_or(1ull << dev, std::memory_order_acq_rel);
+  return e;
+}
+
+template <bool kBf16, int D, int MT, int KS, int kStages, int kPerSm>
+int launch_row(const RowParams &prm, int ctas, cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  auto kernel = paged_row_kernel<kBf16, D, MT, KS, kStages, kPerSm>;
+  constexpr int smem = row_smem_bytes<D, kStages>();
+  TXP_CUDA(allow_smem(kernel, smem, &done));
+  TXP_CUDA(launch(kernel, dim3(ctas), dim3((MT * KS + 1) * 32), smem, stream, prm));
+  return TXD_OK;
+}
+
+template <bool kBf16>
+int launch_row_any(const Plan &plan, const RowParams &prm, cudaStream_t s) {
+  const int mt = plan.shape.mt;
+  // ring: 96 KB a CTA where two share an SM, up to 192 KB where one has it
+  if (plan.kernel_d == 64) {
+    if (mt == 1) return launch_row<kBf16, 64, 1, 4, 6, 2>(prm, plan.ctas, s);
+    if (mt == 2) return launch_row<kBf16, 64, 2, 4, 8, 1>(prm, plan.ctas, s);
+    return launch_row<kBf16, 64, 4, 2, 8, 1>(prm, plan.ctas, s);
+  }
+  if (plan.kernel_d == 128) {
+    if (mt == 1) return launch_row<kBf16, 128, 1, 4, 3, 2>(prm, plan.ctas, s);
+    if (mt == 2) return launch_row<kBf16, 128, 2, 4, 6, 1>(prm, plan.ctas, s);
+    return launch_row<kBf16, 128, 4, 2, 6, 1>(prm, plan.ctas, s);
+  }
+  if (mt == 1) return launch_row<kBf16, 256, 1, 4, 3, 1>(prm, plan.ctas, s);
+  if (mt == 2) return launch_row<kBf16, 256, 2, 4, 3, 1>(prm, plan.ctas, s);
+  return launch_row<kBf16, 256, 4, 2, 3, 1>(prm, plan.ctas, s);
+}
+
+template <typename T>
+int launch_join(const Plan &plan, const JoinParams &j, cudaStream_t s) {
+  if (j.ctas < 2) return TXD_OK;
+  const dim3 grid(j.ctas - 1, (plan.rows + 7) / 8);
+  if (plan.kernel_d == 64) TXP_CUDA(launch(paged_join_kernel<T, 64>, grid, dim3(256), 0, s, j));
+  else if (plan.kernel_d == 128) TXP_CUDA(launch(paged_join_kernel<T, 128>, grid, dim3(256), 0, s, j));
+  else TXP_CUDA(launch(paged_join_kernel<T, 256>, grid, dim3(256), 0, s, j));
+  return TXD_OK;
+}
+
+unsigned long long wait_limit() {
+  unsigned long long ns = 2000ull * 1000 * 1000;
+  if (const char *e = getenv("TXD_WAIT_LIMIT_MS")) {
+    const long ms = atol(e);
+    if (ms > 0) ns = static_cast<unsigned long long>(ms) * 1000 * 1000;
+  }
+  return ns;
+}
+
+}  // namespace
+}  // namespace txp
+
+using namespace txp;
+
+extern "C" {
+
+int64_t tx_paged_attention_workspace(const tx_paged_view *cache, const tx_paged_attn_problem *pr) {
+  Plan plan;
+  if (make_plan(cache, pr, &plan)) return 0;
+  return plan.bytes();
+}
+
+int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_problem *pr, void *workspace, int64_t workspace_bytes,
+                       void *stream_v) {
+  Plan plan;
+  int rc = make_plan(cache, pr, &plan);
+  if (rc) return rc;
+  if (pr->tokens == 0 || plan.view.batch == 0) return TXD_OK;
+  if (!pr->q || !pr->out) return fail(TXD_ERR_INVALID, "null tensor pointer");
+  if ((reinterpret_cast<uintptr_t>(pr->q) | reinterpret_cast<uintptr_t>(pr->out)) & 15)
+    return fail(TXD_ERR_INVALID, "q and out must be 16-byte aligned");
+  int64_t q_stride[2], o_stride[2];
+  for (int i = 0; i < 2; ++i) {
+    const bool one = (i == 0 ? pr->tokens : pr->q_heads) == 1;
+    q_stride[i] = one ? plan.view.head_dim : pr->q_stride[i];
+    o_stride[i] = one ? plan.view.head_dim : pr->out_stride[i];
+    if (q_stride[i] < 0 || o_stride[i] < 0 || q_stride[i] % 8 || o_stride[i] % 8)
+      return fail(TXD_ERR_UNSUPPORTED, "strides of q and out must be non-negative multiples of 16 bytes");
+  }
+  uint32_t *status = nullptr;
+  if ((rc = device_ready(&status))) return rc;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes())
+    return fail(TXD_ERR_INVALID, "a 16-byte aligned workspace of %lld bytes is wanted", static_cast<long long>(plan.bytes()));
+  const tx_paged_view &c = plan.view;
+  char *ws = static_cast<char *>(workspace);
+
+  Sched sched = {};
+  sched.kv_lens = c.kv_lens;
+  sched.cu_q = c.cu_q;
+  sched.batch = c.batch;
+  sched.tokens = pr->tokens;
+  sched.kv_heads = c.kv_heads;
+  sched.group = plan.group;
+  sched.tile_tokens = plan.rows / plan.group;
+  sched.causal = pr->causal ? 1 : 0;
+  sched.window = pr->window > (1 << 30) ? 1 << 30 : pr->window;
+  sched.max_kv = c.table_width * c.page_size;
+  sched.block_shift = 6;
+  sched.tile_cost = 2;
+  sched.min_part = 2;
+  sched.min_share = 4;
+  sched.status = status;
+
+  RowParams prm = {};
+  const int box_rows = c.page_size < 64 ? c.page_size : 64;
+  if ((rc = encode_pool(&prm.tmap_k, c.k, c, c.k_stride, box_rows))) return rc;
+  if ((rc = encode_pool(&prm.tmap_v, c.v, c, c.v_stride, box_rows))) return rc;
+  prm.s = sched;
+  prm.q = pr->q;
+  prm.out = pr->out;
+  prm.m_out = pr->m;
+  for (int i = 0; i < 2; ++i) prm.q_stride[i] = q_stride[i], prm.out_stride[i] = o_stride[i];
+  prm.table = c.table;
+  prm.table_stride = c.table_stride;
+  prm.borders = reinterpret_cast<int4 *>(ws);
+  prm.part = reinterpret_cast<float *>(ws + plan.borders_bytes);
+  prm.ml = reinterpret_cast<float2 *>(ws + plan.borders_bytes + plan.part_bytes);
+  prm.wait_limit_ns = wait_limit();
+  prm.qk_scale = pr->sm_scale * 1.44269504f;  // 1 / ln 2
+  prm.num_pages = c.num_pages;
+  prm.page_shift = shift_of(c.page_size);
+  prm.box_shift = shift_of(box_rows);
+  prm.heads = pr->q_heads;
+  prm.head_dim = c.head_dim;
+  if (const char *e = getenv("TXD_INJECT_STALL")) prm.inject_stall = atoi(e) != 0;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  const bool bf16 = c.dtype == TXD_BF16;
+  if ((rc = bf16 ? launch_row_any<true>(plan, prm, stream) : launch_row_any<false>(plan, prm, stream))) return rc;
+
+  JoinParams join = {};
+  join.s = sched;
+  join.borders = prm.borders;
+  join.part = prm.part;
+  join.ml = prm.ml;
+  join.out = pr->out;
+  join.m_out = pr->m;
+  join.out_stride[0] = o_stride[0];
+  join.out_stride[1] = o_stride[1];
+  join.ctas = plan.ctas;
+  join.rows = plan.rows;
+  join.heads = pr->q_heads;
+  join.head_dim = c.head_dim;
+  if ((rc = bf16 ? launch_join<__nv_bfloat16>(plan, join, stream) : launch_join<__half>(plan, join, stream))) return rc;
+  count_launches(2);
+  return TXD_OK;
+}
+
+}  // extern "C"

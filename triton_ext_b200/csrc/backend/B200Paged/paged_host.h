@@ -24,7 +24,9 @@ int fail(int code, const char *fmt, ...);
 void count_launches(int n);
 // TXD_OK on an sm_100 device; *status receives the device address of its status word.
 int device_ready(uint32_t **status);
-int check_view(const tx_paged_view *c);
+// Checks a caller's view of a cache and copies it to *out in normal form.
+int check_view(const tx_paged_view *c, tx_paged_view *out);
+int shift_of(int page_size);  // log2
 
 #define TXP_CUDA(expr)                                                                            \
   do {                                                                                            \

@@ -1,9 +1,10 @@
 """A cache of keys and values in pages, and what a serving step does with it (include/b200_paged.h):
 
   append            the new tokens' k (turned by their positions) and v into their pages, and the turned q
+  paged_attention   the new tokens' attention over their sequences' pages: chunks of a prompt, drafted tokens, single tokens
   PagedCache        who holds which page, on the device: reserve, fork, free, compact, copy_pages
 
-A step is `cache.reserve(rows, counts)`, then for every layer `append`. Nothing in a step
+A step is `cache.reserve(rows, counts)`, then for every layer `append` and `paged_attention`. Nothing in a step
 synchronises, reads the device or depends on the host knowing a length, so a step can be captured in a CUDA graph and
 replayed while the sequences grow. What kernels find wrong (a bad page, no free pages) is reported by `check`.
 
@@ -34,6 +35,8 @@ def _lib() -> ctypes.CDLL:
         vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
         for name, args, res in (
                 ("tx_paged_append", [vp, vp, vp, vp], ctypes.c_int),
+                ("tx_paged_attention", [vp, vp, vp, i64, vp], ctypes.c_int),
+                ("tx_paged_attention_workspace", [vp, vp], i64),
                 ("tx_pages_workspace", [vp, i32], i64),
                 ("tx_pages_free", [vp, vp, i32, vp], ctypes.c_int),
                 ("tx_pages_fork", [vp, vp, vp, i32, vp, vp], ctypes.c_int),
@@ -62,6 +65,7 @@ def kernel_launches() -> int:
 
 _VIEW = struct.Struct("2P6qPq2P8i")
 _APPEND = struct.Struct("4P8q2i")
+_ATTN = struct.Struct("3P4q5if")
 _STATE = struct.Struct("2Pq3P6i")
 
 
@@ -143,6 +147,50 @@ def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages:
     if rc:
         _raise(lib, rc)
     return out
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    kv_lens: torch.Tensor, sm_scale: float, *, cu_q: Optional[torch.Tensor] = None,
+                    max_q: Optional[int] = None, causal: bool = True, window: int = 0, out: Optional[torch.Tensor] = None,
+                    return_m: bool = False):
+    """Attention of new tokens over their sequences' pages, on the current CUDA stream; see `append` for the arguments that
+    describe the cache and the batch.
+
+    q: [tokens, heads, head_dim], heads a multiple of kv_heads (query head h reads key head h // (heads // kv_heads)). A new
+    token sees the keys up to its own position (all keys of its sequence if not `causal`), with `window` > 0 the last `window`
+    of them. max_q: a bound on the new tokens of one sequence, needed with cu_q. A row that sees nothing gives zeros.
+    Returns the output, with `return_m` also [tokens, heads] fp32 of max + log2(sum) (base 2), -inf where nothing is seen.
+    Rows behind cu_q[-1] are left alone."""
+    lib = _lib()
+    if not q.is_cuda:
+        _not_cuda(q)
+    device = q.device
+    view = _view(k_pages, v_pages, page_table, kv_lens, cu_q, device)
+    tokens, heads, d = q.shape if q.dim() == 3 else _invalid("q must be [tokens, heads, head_dim]")
+    if d != k_pages.shape[3]:
+        _invalid(f"q has head_dim {d}, the cache {k_pages.shape[3]}")
+    qs = _token_strides(q, "q", tokens, d, k_pages)
+    if cu_q is None:
+        if tokens != page_table.shape[0]:
+            _invalid(f"without cu_q there is one new token for each of the {page_table.shape[0]} sequences, got {tokens}")
+        max_q = 1
+    elif max_q is None:
+        _invalid("cu_q needs max_q, a bound on the new tokens of one sequence")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    elif out.shape != q.shape or (tokens > 1 and out.stride(0) == 0) or (heads > 1 and out.stride(1) == 0):
+        _invalid("out must have the shape of q and not be an expanded tensor")
+    os_ = _token_strides(out, "out", tokens, d, k_pages)
+    m = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_m else None
+    problem = _ATTN.pack(q.data_ptr(), out.data_ptr(), m.data_ptr() if return_m else 0, qs[0], qs[1], os_[0], os_[1], tokens,
+                         heads, max_q, int(causal), window, sm_scale)
+    with _on(device) as stream:
+        size = lib.tx_paged_attention_workspace(view, problem)
+        ws = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
+        rc = lib.tx_paged_attention(view, problem, ws.data_ptr() if ws is not None else None, size, stream)
+    if rc:
+        _raise(lib, rc)
+    return (out, m) if return_m else out
 
 
 class PagedCache:
