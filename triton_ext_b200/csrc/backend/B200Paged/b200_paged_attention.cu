@@ -5,7 +5,7 @@
 #include <cstdlib>
 #include <mutex>
 
-#include "paged_row_kernel.cuh"
+#include "paged_tile_kernel.cuh"
 
 namespace txp {
 namespace {
@@ -27,9 +27,10 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// One pool as {64 columns, slots, column groups, heads, pages}; a box is `box_rows` slots of one page and head, with all
-// column groups. Columns past head_dim (16 and 32) are out of bounds and arrive as zeros.
-int encode_pool(CUtensorMap *map, const void *ptr, const tx_paged_view &c, const int64_t *stride, int box_rows) {
+// One pool as {64 columns, slots, column groups, heads, pages}; a box is `box_rows` slots of one page and head, with
+// `box_groups` column groups. Columns past head_dim (16 and 32) are out of bounds and arrive as zeros.
+int encode_pool(CUtensorMap *map, const void *ptr, const tx_paged_view &c, const int64_t *stride, int box_rows,
+                int box_groups) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return fail(TXD_ERR_NO_DEVICE, "cuTensorMapEncodeTiled is not available from the CUDA driver");
   const int groups = c.head_dim > 64 ? c.head_dim / 64 : 1;
@@ -37,12 +38,28 @@ int encode_pool(CUtensorMap *map, const void *ptr, const tx_paged_view &c, const
                               static_cast<cuuint64_t>(groups), static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.num_pages)};
   const cuuint64_t strides[4] = {static_cast<cuuint64_t>(stride[1]) * 2, 128, static_cast<cuuint64_t>(stride[2]) * 2,
                                  static_cast<cuuint64_t>(stride[0]) * 2};
-  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(groups), 1, 1};
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(box_groups), 1, 1};
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r = enc(map, c.dtype == TXD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                          const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(TXD_ERR_CUDA, "cuTensorMapEncodeTiled (pool) failed with code %d", static_cast<int>(r));
+  return TXD_OK;
+}
+
+// Queries as {head_dim, heads, tokens}; a box is the heads of one key head of a sub-tile's tokens.
+int encode_queries(CUtensorMap *map, const void *ptr, const tx_paged_view &c, const int64_t *stride, int heads, int tokens,
+                   int group, int sub_tokens) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fail(TXD_ERR_NO_DEVICE, "cuTensorMapEncodeTiled is not available from the CUDA driver");
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride[1]) * 2, static_cast<cuuint64_t>(stride[0]) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(sub_tokens)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, c.dtype == TXD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TXD_ERR_CUDA, "cuTensorMapEncodeTiled (queries) failed with code %d", static_cast<int>(r));
   return TXD_OK;
 }
 
@@ -76,6 +93,7 @@ int sm_count() {
 struct Plan {
   tx_paged_view view;
   int kernel_d, group, rows, ctas;
+  bool tiled;  // the kernel for many rows
   RowShape shape;
   size_t borders_bytes, part_bytes, ml_bytes;
   int64_t bytes() const { return static_cast<int64_t>(borders_bytes + part_bytes + ml_bytes); }
@@ -99,8 +117,11 @@ int make_plan(const tx_paged_view *cache, const tx_paged_attn_problem *pr, Plan 
   int max_q = pr->max_q;
   if (max_q > pr->tokens) max_q = pr->tokens;
   plan->shape = row_shape(plan->kernel_d, plan->group, max_q);
-  plan->rows = plan->shape.mt * 16;
-  plan->ctas = sm_count() * plan->shape.per_sm;
+  // 128-row tiles on tcgen05 for head dimensions up to 128 (256 columns of O for two sub-tiles do not fit tensor memory
+  // next to S); up to 64 rows the streaming kernel
+  plan->tiled = plan->kernel_d <= 128 && static_cast<long long>(plan->group) * max_q > 64;
+  plan->rows = plan->tiled ? 256 : plan->shape.mt * 16;
+  plan->ctas = sm_count() * (plan->tiled ? 1 : plan->shape.per_sm);
   plan->borders_bytes = (static_cast<size_t>(plan->ctas) * 16 + 255) / 256 * 256;
   const size_t rows = static_cast<size_t>(plan->ctas) * 2 * plan->rows;
   plan->part_bytes = rows * plan->kernel_d * 4;
@@ -164,6 +185,26 @@ int launch_row_any(const Plan &plan, const RowParams &prm, cudaStream_t s) {
   if (mt == 1) return launch_row<kBf16, 256, 1, 4, 3, 1>(prm, plan.ctas, s);
   if (mt == 2) return launch_row<kBf16, 256, 2, 4, 3, 1>(prm, plan.ctas, s);
   return launch_row<kBf16, 256, 4, 2, 3, 1>(prm, plan.ctas, s);
+}
+
+template <bool kBf16, int D>
+int launch_tile(const TileParams &prm, int ctas, cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  auto kernel = paged_tile_kernel<kBf16, D>;
+  TXP_CUDA(allow_smem(kernel, TileShape<D>::kSmem, &done));
+  TXP_CUDA(launch(kernel, dim3(ctas), dim3(kTileThreads), TileShape<D>::kSmem, stream, prm));
+  return TXD_OK;
+}
+
+template <bool kBf16>
+int launch_tile_any(const Plan &plan, const TileParams &prm, cudaStream_t s) {
+  return plan.kernel_d == 64 ? launch_tile<kBf16, 64>(prm, plan.ctas, s) : launch_tile<kBf16, 128>(prm, plan.ctas, s);
+}
+
+// tcgen05 instruction descriptor: fp32 accumulator, A and B f16 or bf16, B n-major or k-major, 128 x n
+uint32_t mma_idesc(bool bf16, bool b_mn_major, int n) {
+  const uint32_t type = bf16 ? 1u : 0u;
+  return 1u << 4 | type << 7 | type << 10 | (b_mn_major ? 1u : 0u) << 16 | static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
 }
 
 template <typename T>
@@ -239,37 +280,66 @@ int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_problem *
   sched.min_share = 4;
   sched.status = status;
 
-  RowParams prm = {};
-  const int box_rows = c.page_size < 64 ? c.page_size : 64;
-  if ((rc = encode_pool(&prm.tmap_k, c.k, c, c.k_stride, box_rows))) return rc;
-  if ((rc = encode_pool(&prm.tmap_v, c.v, c, c.v_stride, box_rows))) return rc;
-  prm.s = sched;
-  prm.q = pr->q;
-  prm.out = pr->out;
-  prm.m_out = pr->m;
-  for (int i = 0; i < 2; ++i) prm.q_stride[i] = q_stride[i], prm.out_stride[i] = o_stride[i];
-  prm.table = c.table;
-  prm.table_stride = c.table_stride;
-  prm.borders = reinterpret_cast<int4 *>(ws);
-  prm.part = reinterpret_cast<float *>(ws + plan.borders_bytes);
-  prm.ml = reinterpret_cast<float2 *>(ws + plan.borders_bytes + plan.part_bytes);
-  prm.wait_limit_ns = wait_limit();
-  prm.qk_scale = pr->sm_scale * 1.44269504f;  // 1 / ln 2
-  prm.num_pages = c.num_pages;
-  prm.page_shift = shift_of(c.page_size);
-  prm.box_shift = shift_of(box_rows);
-  prm.heads = pr->q_heads;
-  prm.head_dim = c.head_dim;
-  if (const char *e = getenv("TXD_INJECT_STALL")) prm.inject_stall = atoi(e) != 0;
+  if (plan.tiled) {
+    sched.tile_tokens = 2 * (128 / plan.group);
+    sched.block_shift = 7;
+  }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   const bool bf16 = c.dtype == TXD_BF16;
-  if ((rc = bf16 ? launch_row_any<true>(plan, prm, stream) : launch_row_any<false>(plan, prm, stream))) return rc;
+  int4 *borders = reinterpret_cast<int4 *>(ws);
+  float *part = reinterpret_cast<float *>(ws + plan.borders_bytes);
+  float2 *ml = reinterpret_cast<float2 *>(ws + plan.borders_bytes + plan.part_bytes);
+  const float qk_scale = pr->sm_scale * 1.44269504f;  // 1 / ln 2
+  int32_t inject_stall = 0;
+  if (const char *e = getenv("TXD_INJECT_STALL")) inject_stall = atoi(e) != 0;
+  auto fill = [&](auto &prm, int box_rows) {
+    prm.s = sched;
+    prm.out = pr->out;
+    prm.m_out = pr->m;
+    for (int i = 0; i < 2; ++i) prm.out_stride[i] = o_stride[i];
+    prm.table = c.table;
+    prm.table_stride = c.table_stride;
+    prm.borders = borders;
+    prm.part = part;
+    prm.ml = ml;
+    prm.wait_limit_ns = wait_limit();
+    prm.qk_scale = qk_scale;
+    prm.num_pages = c.num_pages;
+    prm.page_shift = shift_of(c.page_size);
+    prm.box_shift = shift_of(box_rows);
+    prm.heads = pr->q_heads;
+    prm.head_dim = c.head_dim;
+    prm.inject_stall = inject_stall;
+  };
+  if (plan.tiled) {
+    TileParams prm = {};
+    const int box_rows = c.page_size < 128 ? c.page_size : 128;
+    prm.sub_tokens = 128 / plan.group;
+    prm.part_rows = plan.rows;
+    if ((rc = encode_queries(&prm.tmap_q, pr->q, c, q_stride, pr->q_heads, pr->tokens, plan.group, prm.sub_tokens))) return rc;
+    if ((rc = encode_pool(&prm.tmap_k, c.k, c, c.k_stride, box_rows, 1))) return rc;
+    if ((rc = encode_pool(&prm.tmap_v, c.v, c, c.v_stride, box_rows, 1))) return rc;
+    fill(prm, box_rows);
+    prm.idesc_qk = mma_idesc(bf16, false, 128);
+    prm.idesc_pv = mma_idesc(bf16, true, plan.kernel_d);
+    if ((rc = bf16 ? launch_tile_any<true>(plan, prm, stream) : launch_tile_any<false>(plan, prm, stream))) return rc;
+  } else {
+    RowParams prm = {};
+    const int box_rows = c.page_size < 64 ? c.page_size : 64;
+    const int groups = plan.kernel_d / 64;
+    if ((rc = encode_pool(&prm.tmap_k, c.k, c, c.k_stride, box_rows, groups))) return rc;
+    if ((rc = encode_pool(&prm.tmap_v, c.v, c, c.v_stride, box_rows, groups))) return rc;
+    fill(prm, box_rows);
+    prm.q = pr->q;
+    for (int i = 0; i < 2; ++i) prm.q_stride[i] = q_stride[i];
+    if ((rc = bf16 ? launch_row_any<true>(plan, prm, stream) : launch_row_any<false>(plan, prm, stream))) return rc;
+  }
 
   JoinParams join = {};
   join.s = sched;
-  join.borders = prm.borders;
-  join.part = prm.part;
-  join.ml = prm.ml;
+  join.borders = borders;
+  join.part = part;
+  join.ml = ml;
   join.out = pr->out;
   join.m_out = pr->m;
   join.out_stride[0] = o_stride[0];
