@@ -93,22 +93,21 @@ struct Widest {
 };
 
 template <typename T>
-int launch_rotary_t(RotaryParams &prm, int v, cudaStream_t stream) {
-  const size_t smem = sizeof(float2) * prm.block_tokens * (prm.rope.rotary_dim / 2);
-  const long long blocks = (prm.total + prm.block_tokens - 1) / prm.block_tokens;
-  if (blocks > INT_MAX) return fail(TXD_ERR_UNSUPPORTED, "too many tokens for one launch");
-  const unsigned grid = static_cast<unsigned>(blocks);
+int launch_rotary_t(const RotaryParams &prm, int v, cudaStream_t stream) {
+  const long long warps = static_cast<long long>(prm.total) * prm.slices;
+  const unsigned grid = static_cast<unsigned>((warps + kRotaryThreads / 32 - 1) / (kRotaryThreads / 32));
   constexpr int kWide = 16 / static_cast<int>(sizeof(T));
-  if (v == kWide) rotary_kernel<T, kWide><<<grid, kRotaryThreads, smem, stream>>>(prm);
-  else if (v >= 2) rotary_kernel<T, 2><<<grid, kRotaryThreads, smem, stream>>>(prm);
-  else rotary_kernel<T, 1><<<grid, kRotaryThreads, smem, stream>>>(prm);
+  if (v == kWide) rotary_kernel<T, kWide><<<grid, kRotaryThreads, 0, stream>>>(prm);
+  else if (v >= 2) rotary_kernel<T, 2><<<grid, kRotaryThreads, 0, stream>>>(prm);
+  else rotary_kernel<T, 1><<<grid, kRotaryThreads, 0, stream>>>(prm);
   TXP_CUDA(cudaGetLastError());
   count_launches(1);
   return TXD_OK;
 }
 
-// Units, vector width, tokens per block; then the launch. prm.part[].units holds the part's heads on entry.
-int launch_rotary(RotaryParams &prm, const int *heads, int head_dim, int dtype, cudaStream_t stream) {
+// Vector width, lanes of a head, warps of a token; then the launch.
+int launch_rotary(RotaryParams &prm, long long total, int head_dim, int dtype, cudaStream_t stream) {
+  if (total > INT_MAX) return fail(TXD_ERR_UNSUPPORTED, "%lld tokens: at most 2^31 - 1 in one launch", total);
   const int size = dtype == TXD_F32 ? 4 : 2;
   const int rd = prm.rope.rotary_dim;
   Widest w{16 / size};
@@ -125,27 +124,25 @@ int launch_rotary(RotaryParams &prm, const int *heads, int head_dim, int dtype, 
   w.divide(head_dim - rd);
   w.divide(head_dim);
   if (w.v != 16 / size && w.v > 2) w.v = 2;
-  long long units = 0;
+  prm.turned = rd / 2 / w.v;
+  int most = 1;  // steps over the heads of the part that takes the most
   for (int i = 0; i < prm.parts; ++i) {
     RotaryPart &q = prm.part[i];
-    q.first_unit = static_cast<int32_t>(units);
-    q.turned = q.kind == kCopyToPage ? 0 : rd / 2 / w.v;
-    const int from = q.turned ? rd : 0;
-    // in place, the columns behind the rotated ones stand where they belong already
+    // in place, the columns behind the turned ones stand where they belong already
     const bool same = q.kind == kTurn && q.in == q.out && q.in_stride[0] == q.out_stride[0] &&
                       q.in_stride[1] == q.out_stride[1] && q.in_stride[2] == q.out_stride[2];
-    q.units = q.turned + (same ? 0 : (head_dim - from) / w.v);
-    units += static_cast<long long>(heads[i]) * q.units;
+    q.pass = q.kind == kCopyToPage ? head_dim / w.v : same ? 0 : (head_dim - rd) / w.v;
+    const int units = (q.kind == kCopyToPage ? 0 : prm.turned) + q.pass;
+    while ((1 << q.lanes_shift) < units && q.lanes_shift < 5) ++q.lanes_shift;
+    const int steps = (q.heads * (1 << q.lanes_shift) + 31) / 32;
+    if (steps > most) most = steps;
   }
-  if (units > (1 << 24)) return fail(TXD_ERR_UNSUPPORTED, "too many heads for one token");
-  prm.units = static_cast<int32_t>(units);
-  // Tokens per block: enough that every thread has its kUnroll vectors in flight at once, as long as the blocks still
-  // cover the SMs several times over.
-  int bt = static_cast<int>(kRotaryThreads * kUnroll / (units > 0 ? units : 1));
-  if (bt < 1) bt = 1;
-  if (bt > kMaxBlockTokens) bt = kMaxBlockTokens;
-  while (bt > 1 && prm.total / bt < 148 * 4) bt /= 2;
-  prm.block_tokens = bt;
+  // A warp takes a whole token where there are tokens enough to fill the SMs (32 warps each); fewer tokens are shared.
+  long long slices = total > 0 ? 148ll * 32 * 2 / total : 1;
+  if (slices > most) slices = most;
+  if (slices < 1) slices = 1;
+  prm.slices = static_cast<uint32_t>(slices);
+  prm.total = static_cast<uint32_t>(total);
   if (dtype == TXD_F32) return launch_rotary_t<float>(prm, w.v, stream);
   if (dtype == TXD_BF16) return launch_rotary_t<__nv_bfloat16>(prm, w.v, stream);
   return launch_rotary_t<__half>(prm, w.v, stream);
@@ -229,16 +226,18 @@ int tx_rotary(const tx_rope *rope, const tx_rotary_problem *pr, const void *posi
   if (!rope || !pr) return fail(TXD_ERR_INVALID, "null argument");
   if (pr->dtype != TXD_F16 && pr->dtype != TXD_BF16 && pr->dtype != TXD_F32)
     return fail(TXD_ERR_UNSUPPORTED, "rotary takes f16, bf16 or f32");
+  if (pr->head_dim > 1024) return fail(TXD_ERR_UNSUPPORTED, "head_dim %d: at most 1024", pr->head_dim);
   if (pr->batch < 0 || pr->tokens < 0 || pr->head_dim < 1 || pr->parts < 1 || pr->parts > 2)
     return fail(TXD_ERR_INVALID, "batch, tokens must be >= 0, head_dim >= 1, parts 1 or 2");
   int rc = check_rope(rope, pr->head_dim);
   if (rc) return rc;
   RotaryParams prm = {};
-  int heads[3] = {};
+  int heads = 0;
   for (int i = 0; i < pr->parts; ++i) {
     const tx_rotary_part &q = pr->part[i];
     if (q.heads < 0) return fail(TXD_ERR_INVALID, "negative heads");
-    heads[i] = q.heads;
+    heads |= q.heads;
+    prm.part[i].heads = q.heads;
     prm.part[i].in = q.in;
     prm.part[i].out = q.out;
     for (int j = 0; j < 3; ++j) {
@@ -248,10 +247,10 @@ int tx_rotary(const tx_rope *rope, const tx_rotary_problem *pr, const void *posi
     prm.part[i].kind = kTurn;
   }
   const long long total = static_cast<long long>(pr->batch) * pr->tokens;
-  if (total == 0 || heads[0] + heads[1] == 0) return TXD_OK;
+  if (total == 0 || heads == 0) return TXD_OK;
   if (!positions) return fail(TXD_ERR_INVALID, "null positions");
   for (int i = 0; i < pr->parts; ++i)
-    if (heads[i] > 0 && (!pr->part[i].in || !pr->part[i].out)) return fail(TXD_ERR_INVALID, "null tensor pointer");
+    if (pr->part[i].heads > 0 && (!pr->part[i].in || !pr->part[i].out)) return fail(TXD_ERR_INVALID, "null tensor pointer");
   if ((rc = device_ready(&prm.status))) return rc;
   prm.rope = *rope;
   prm.positions = positions;
@@ -259,10 +258,9 @@ int tx_rotary(const tx_rope *rope, const tx_rotary_problem *pr, const void *posi
   prm.position_stride[0] = pr->position_stride[0];
   prm.position_stride[1] = pr->position_stride[1];
   prm.inverse = pr->inverse;
-  prm.total = total;
-  prm.tokens = pr->tokens;
+  prm.tokens = static_cast<uint32_t>(pr->tokens);
   prm.parts = pr->parts;
-  return launch_rotary(prm, heads, pr->head_dim, pr->dtype, static_cast<cudaStream_t>(stream));
+  return launch_rotary(prm, total, pr->head_dim, pr->dtype, static_cast<cudaStream_t>(stream));
 }
 
 int tx_paged_append(const tx_paged_view *cache, const tx_rope *rope, const tx_append_problem *pr, void *stream) {
@@ -279,7 +277,7 @@ int tx_paged_append(const tx_paged_view *cache, const tx_rope *rope, const tx_ap
   if ((rc = device_ready(&prm.status))) return rc;
   if (rope) prm.rope = *rope;
   else prm.rope.rotary_dim = 0, prm.rope.magnitude = 1.f;
-  int heads[3] = {}, n = 0;
+  int n = 0;
   auto part = [&](const void *in, const int64_t *in_s, void *out, const int64_t *out_s, int kind, int h) {
     RotaryPart &q = prm.part[n];
     q.in = in;
@@ -289,7 +287,8 @@ int tx_paged_append(const tx_paged_view *cache, const tx_rope *rope, const tx_ap
     if (kind == kTurn) q.out_stride[1] = out_s[1], q.out_stride[2] = out_s[0];
     else for (int j = 0; j < 3; ++j) q.out_stride[j] = out_s[j];
     q.kind = kind;
-    heads[n++] = h;
+    q.heads = h;
+    ++n;
   };
   // without a rotation, a q that is its own output has nothing to be done to it
   const bool idle_q = !rope && pr->q == pr->q_out && pr->q_stride[0] == pr->q_out_stride[0] && pr->q_stride[1] == pr->q_out_stride[1];
@@ -305,9 +304,8 @@ int tx_paged_append(const tx_paged_view *cache, const tx_rope *rope, const tx_ap
   prm.table_width = c->table_width;
   prm.num_pages = c->num_pages;
   prm.page_shift = shift_of(c->page_size);
-  prm.total = pr->tokens;
-  prm.tokens = pr->tokens;
-  return launch_rotary(prm, heads, c->head_dim, c->dtype, static_cast<cudaStream_t>(stream));
+  prm.tokens = static_cast<uint32_t>(pr->tokens);
+  return launch_rotary(prm, pr->tokens, c->head_dim, c->dtype, static_cast<cudaStream_t>(stream));
 }
 
 int64_t tx_pages_workspace(const tx_pages_state *st, int32_t n) {

@@ -3,11 +3,15 @@
 // Pair i of a head is the complex number x1 + i x2; a position p turns it by the angle 2 pi p f_i, where f_i is kept as
 // a 64-bit fraction of a turn. p * f_i in 64-bit wrap-around arithmetic IS the angle modulo whole turns, so no range
 // reduction loses anything at far positions (a product in fp32 is off by 0.06 rad at position 2^20 already); its upper
-// 32 bits go through sincospi. The cosines and sines of a token are computed once per block and used by all heads.
+// 32 bits go through sincospi.
 //
 // The work is one read and one write of every value: HBM bound when there are many tokens, launch bound when there are
-// few. A block takes a few tokens, so that every thread has up to kUnroll pairs of vectors in flight before the block
-// looks at positions and computes angles; the loads do not depend on either.
+// few. A warp takes one token (a slice of its heads when there are few tokens): its lanes are the vectors of a head, by as
+// many heads as fit 32 lanes, and step over the rest, so a lane keeps the cosines and sines of its V pairs in registers for
+// all heads. The warp computes each angle once and passes it on through its own piece of shared memory. Warps never wait for
+// one another. (A block per few tokens with the angles in shared memory, two barriers apart from its loads,
+// took 229 us for the training case, 4 x 4096 tokens of 40 heads
+// of 128 bf16 forward and backward; this takes 114 us, 5.9 TB/s.)
 #pragma once
 
 #include <cuda_bf16.h>
@@ -18,8 +22,7 @@
 namespace txp {
 
 constexpr int kRotaryThreads = 256;
-constexpr int kMaxBlockTokens = 8;
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 2;  // heads whose vectors a lane has in flight
 
 enum RotaryKind : int32_t { kTurn = 0, kTurnToPage = 1, kCopyToPage = 2 };
 
@@ -28,8 +31,9 @@ struct RotaryPart {
   void *out;               // kTurn: the tensor; else the pool
   long long in_stride[3];  // batch, head, token
   long long out_stride[3]; // kTurn: batch, head, token; else page, slot, head
-  int32_t kind, first_unit;
-  int32_t turned, units;   // units of a head: `turned` pairs of vectors, then single vectors that pass
+  int32_t kind, heads;
+  int32_t pass;            // vectors of a head behind the turned columns that have to be copied
+  int32_t lanes_shift;     // log2 of the lanes that one head takes (at most 5)
 };
 
 struct RotaryParams {
@@ -40,8 +44,10 @@ struct RotaryParams {
   const int32_t *table, *kv_lens, *cu_q;
   long long table_stride;
   uint32_t *status;
-  long long total;         // tokens of all batch entries
-  int32_t tokens, parts, units, block_tokens, positions_64, inverse;
+  uint32_t total;          // tokens of all batch entries
+  uint32_t tokens, slices; // slices: warps that share a token's heads
+  int32_t parts, turned;   // turned: pairs of vectors of a head
+  int32_t positions_64, inverse;
   int32_t batch, table_width, num_pages, page_shift;
 };
 
@@ -50,163 +56,180 @@ struct alignas(sizeof(T) * V) Pack {
   T x[V];
 };
 
-__device__ __forceinline__ float rot_f32(float x) { return x; }
-__device__ __forceinline__ float rot_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float rot_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+// Turns the V pairs in a and b by (c, s): pairs (a[e], b[e]), or neighbours of the sequence a, b when interleaved. 16-bit
+// values are taken two to a word: with one value at a time, extracting and packing took more instructions than the rest
+// (training case: 196 us, against 121).
 template <typename T>
-__device__ __forceinline__ T rot_from(float x);
+struct Word;
 template <>
-__device__ __forceinline__ float rot_from<float>(float x) { return x; }
+struct Word<__half> {
+  static __device__ __forceinline__ float2 up(uint32_t w) { return __half22float2(*reinterpret_cast<__half2 *>(&w)); }
+  static __device__ __forceinline__ uint32_t down(float x, float y) {
+    __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<uint32_t *>(&h);
+  }
+  static __device__ __forceinline__ float one(__half x) { return __half2float(x); }
+  static __device__ __forceinline__ __half back(float x) { return __float2half_rn(x); }
+};
 template <>
-__device__ __forceinline__ __half rot_from<__half>(float x) { return __float2half_rn(x); }
+struct Word<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 up(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t down(float x, float y) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<uint32_t *>(&h);
+  }
+  static __device__ __forceinline__ float one(__nv_bfloat16 x) { return __bfloat162float(x); }
+  static __device__ __forceinline__ __nv_bfloat16 back(float x) { return __float2bfloat16_rn(x); }
+};
 template <>
-__device__ __forceinline__ __nv_bfloat16 rot_from<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+struct Word<float> {
+  static __device__ __forceinline__ float one(float x) { return x; }
+  static __device__ __forceinline__ float back(float x) { return x; }
+};
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  extern __shared__ float2 turn[];  // [block_tokens][rotary_dim / 2]: cosine, sine
-  __shared__ long long s_pos[kMaxBlockTokens];
-  __shared__ int s_page[kMaxBlockTokens], s_seq[kMaxBlockTokens];
-  const long long t0 = static_cast<long long>(blockIdx.x) * p.block_tokens;
-  const int here = static_cast<int>(min(static_cast<long long>(p.block_tokens), p.total - t0));
-  const int all = here * p.units;
-  const int half_dim = p.rope.rotary_dim / 2;
-  const bool append = p.positions == nullptr;
-  const int slots = 1 << p.page_shift;
+__device__ __forceinline__ void turn_pairs(Pack<T, V> &a, Pack<T, V> &b, const float2 (&cs)[V], bool interleaved) {
+  if constexpr (sizeof(T) == 2 && V > 1) {
+    uint32_t (&x)[V / 2] = *reinterpret_cast<uint32_t (*)[V / 2]>(&a);
+    uint32_t (&y)[V / 2] = *reinterpret_cast<uint32_t (*)[V / 2]>(&b);
+    if (interleaved) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        uint32_t &w = i < V / 2 ? x[i] : y[i - V / 2];
+        const float2 v = Word<T>::up(w);
+        w = Word<T>::down(v.x * cs[i].x - v.y * cs[i].y, v.y * cs[i].x + v.x * cs[i].y);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const float2 u = Word<T>::up(x[i]), v = Word<T>::up(y[i]), c0 = cs[2 * i], c1 = cs[2 * i + 1];
+        x[i] = Word<T>::down(u.x * c0.x - v.x * c0.y, u.y * c1.x - v.y * c1.y);
+        y[i] = Word<T>::down(v.x * c0.x + u.x * c0.y, v.y * c1.x + u.y * c1.y);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      T &first = !interleaved ? a.x[i] : 2 * i < V ? a.x[2 * i] : b.x[2 * i - V];
+      T &second = !interleaved ? b.x[i] : 2 * i + 1 < V ? a.x[2 * i + 1] : b.x[2 * i + 1 - V];
+      const float x1 = Word<T>::one(first), x2 = Word<T>::one(second);
+      first = Word<T>::back(x1 * cs[i].x - x2 * cs[i].y);
+      second = Word<T>::back(x2 * cs[i].x + x1 * cs[i].y);
+    }
+  }
+}
 
-  for (int base = 0; base < all; base += kRotaryThreads * kUnroll) {
-    Pack<T, V> a[kUnroll], b[kUnroll];
-    int where[kUnroll], head[kUnroll];  // where: part | token << 2 | unit << 8
-#pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      const int u = base + j * kRotaryThreads + static_cast<int>(threadIdx.x);
-      where[j] = -1;
-      if (u >= all) continue;
-      const int tok = u / p.units;
-      int rest = u - tok * p.units;
-      int part = 0;
-      if (p.parts > 1 && rest >= p.part[1].first_unit) part = 1;
-      if (p.parts > 2 && rest >= p.part[2].first_unit) part = 2;
-      const RotaryPart &q = p.part[part];
-      rest -= q.first_unit;
-      const int h = rest / q.units, k = rest - h * q.units;
-      where[j] = part | tok << 2 | k << 8;
-      head[j] = h;
-      const long long t = t0 + tok;
-      const long long z = append ? 0 : t / p.tokens;
-      const T *src = static_cast<const T *>(q.in) + z * q.in_stride[0] + h * q.in_stride[1] + (t - z * p.tokens) * q.in_stride[2];
-      if (k < q.turned) {
-        const int c1 = p.rope.interleaved ? 2 * k * V : k * V;
-        const int c2 = p.rope.interleaved ? c1 + V : c1 + half_dim;
-        a[j] = *reinterpret_cast<const Pack<T, V> *>(src + c1);
-        b[j] = *reinterpret_cast<const Pack<T, V> *>(src + c2);
-      } else {
-        a[j] = *reinterpret_cast<const Pack<T, V> *>(src + (q.turned ? p.rope.rotary_dim : 0) + (k - q.turned) * V);
-      }
+// The last entry of cu[0 .. n] that is at most t, by 32 probes a step.
+__device__ __forceinline__ int find_sequence(const int32_t *cu, int n, int t, int lane) {
+  int lo = 0, left = n + 1;
+  while (left > 1) {
+    const int step = (left + 31) / 32;
+    const int at = lo + lane * step;
+    const uint32_t below = __ballot_sync(0xffffffffu, lane * step < left && cu[min(at, n)] <= t);
+    const int hit = below ? 31 - __clz(below) : 0;
+    lo += hit * step;
+    left = min(step, left - hit * step);
+  }
+  return lo;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kRotaryThreads, 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  // cosine and sine of pair k * V + i at [i][k]: the lanes of a head read neighbouring banks
+  __shared__ float2 s_turn[kRotaryThreads / 32][TX_ROPE_MAX_PAIRS];
+  float2 *turn = s_turn[threadIdx.x >> 5];
+  const int lane = threadIdx.x & 31;
+  const uint32_t id = blockIdx.x * (kRotaryThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t t = p.slices == 1 ? id : id / p.slices;
+  if (t >= p.total) return;
+  const int slice = static_cast<int>(id - t * p.slices);
+  const bool append = p.positions == nullptr;
+  // ---- the token's position, and where an append puts it ----
+  long long pos, page = -1, z = 0, n = t;
+  if (append) {
+    const int s = p.cu_q ? find_sequence(p.cu_q, p.batch, static_cast<int>(t), lane) : static_cast<int>(t);
+    if (s >= p.batch || (p.cu_q && p.cu_q[0] > static_cast<int>(t))) return;  // behind the last sequence
+    pos = p.cu_q ? static_cast<long long>(p.kv_lens[s]) - (p.cu_q[s + 1] - static_cast<int>(t)) : p.kv_lens[s] - 1;
+    uint32_t bad = 0;
+    if (pos < 0) {
+      bad = kBadLength;
+    } else if ((pos >> p.page_shift) >= p.table_width) {
+      bad = kNoRoomInRow;
+    } else {
+      page = p.table[s * p.table_stride + (pos >> p.page_shift)];
+      if (page < 0 || page >= p.num_pages) bad = kBadPage, page = -1;
     }
-    if (base == 0) {
-      if (append) {
-        // the sequence of each token, found by all threads at once; tokens behind the last sequence keep -1
-        if (threadIdx.x < kMaxBlockTokens) s_seq[threadIdx.x] = -1;
-        __syncthreads();
-        if (p.cu_q) {
-          for (int s = threadIdx.x; s < p.batch; s += kRotaryThreads) {
-            const long long lo = p.cu_q[s], hi = p.cu_q[s + 1];
-            for (int i = 0; i < here; ++i)
-              if (t0 + i >= lo && t0 + i < hi) s_seq[i] = s;
-          }
-        } else if (threadIdx.x < here) {
-          s_seq[threadIdx.x] = t0 + threadIdx.x < p.batch ? static_cast<int>(t0 + threadIdx.x) : -1;
-        }
-        __syncthreads();
-        if (threadIdx.x < here) {
-          const int s = s_seq[threadIdx.x];
-          int page = -1;
-          if (s >= 0) {
-            const long long t = t0 + threadIdx.x;
-            const long long pos = p.cu_q ? p.kv_lens[s] - (p.cu_q[s + 1] - t) : p.kv_lens[s] - 1;
-            s_pos[threadIdx.x] = pos;
-            if (pos < 0) {
-              atomicOr(p.status, kBadLength);
-            } else if ((pos >> p.page_shift) >= p.table_width) {
-              atomicOr(p.status, kNoRoomInRow);
-            } else {
-              page = p.table[s * p.table_stride + (pos >> p.page_shift)];
-              if (page < 0 || page >= p.num_pages) {
-                atomicOr(p.status, kBadPage);
-                page = -1;
-              }
-            }
-          } else {
-            s_pos[threadIdx.x] = 0;
-          }
-          s_page[threadIdx.x] = page;
-        }
-      } else if (threadIdx.x < here) {
-        const long long t = t0 + threadIdx.x, z = t / p.tokens;
-        const long long at = z * p.position_stride[0] + (t - z * p.tokens) * p.position_stride[1];
-        s_pos[threadIdx.x] = p.positions_64 ? static_cast<const long long *>(p.positions)[at]
-                                            : static_cast<long long>(static_cast<const int32_t *>(p.positions)[at]);
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < here * half_dim; i += kRotaryThreads) {
-        const int tok = i / half_dim, pair = i - tok * half_dim;
-        const unsigned long long angle = static_cast<unsigned long long>(s_pos[tok]) * p.rope.turns[pair];
-        float s, c;
-        sincospif(static_cast<float>(static_cast<int32_t>(angle >> 32)) * 0x1p-31f, &s, &c);
-        turn[i] = make_float2(c * p.rope.magnitude, (p.inverse ? -s : s) * p.rope.magnitude);
-      }
-      __syncthreads();
+    if (bad && lane == 0) atomicOr(p.status, bad);
+  } else {
+    z = t / p.tokens;
+    n = t - static_cast<uint32_t>(z) * p.tokens;
+    const long long at = z * p.position_stride[0] + n * p.position_stride[1];
+    pos = p.positions_64 ? static_cast<const long long *>(p.positions)[at]
+                         : static_cast<long long>(static_cast<const int32_t *>(p.positions)[at]);
+  }
+  const int slot = static_cast<int>(pos & ((1ll << p.page_shift) - 1));
+  const int half_dim = p.rope.rotary_dim / 2;
+  // read through a generic address: the lanes' words are neighbours, which the constant port would serve one after another
+  // (121 us instead of 114 for the training case)
+  const uint64_t *turns_at = p.rope.turns;
+  asm volatile("" : "+l"(turns_at));
+  for (int i = lane; i < half_dim; i += 32) {
+    const unsigned long long angle = static_cast<unsigned long long>(pos) * turns_at[i];
+    float c, s;
+    sincospif(static_cast<float>(static_cast<int32_t>(angle >> 32)) * 0x1p-31f, &s, &c);
+    turn[(i % V) * p.turned + i / V] = make_float2(c * p.rope.magnitude, (p.inverse ? -s : s) * p.rope.magnitude);
+  }
+  __syncwarp();
+
+  for (int i = 0; i < p.parts; ++i) {
+    const RotaryPart &q = p.part[i];
+    if (q.kind != kTurn && page < 0) continue;
+    const T *src = static_cast<const T *>(q.in) + z * q.in_stride[0] + n * q.in_stride[2];
+    T *dst = static_cast<T *>(q.out);
+    long long dst_head;
+    if (q.kind == kTurn) {
+      dst += z * q.out_stride[0] + n * q.out_stride[2];
+      dst_head = q.out_stride[1];
+    } else {
+      dst += page * q.out_stride[0] + slot * q.out_stride[1];
+      dst_head = q.out_stride[2];
     }
+    const int turned = q.kind == kCopyToPage ? 0 : p.turned, from = q.kind == kCopyToPage ? 0 : p.rope.rotary_dim;
+    const int lanes = 1 << q.lanes_shift, hl = lane >> q.lanes_shift, beside = 32 >> q.lanes_shift;
+    for (int k0 = 0; k0 < turned + q.pass; k0 += lanes) {
+      const int k = k0 + (lane & (lanes - 1));
+      const bool turns = k < turned, active = k < turned + q.pass;
+      float2 cs[V];
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      if (where[j] < 0) continue;
-      const int part = where[j] & 3, tok = (where[j] >> 2) & 63, k = where[j] >> 8;
-      const RotaryPart &q = p.part[part];
-      T *dst = static_cast<T *>(q.out);
-      const long long t = t0 + tok;
-      if (q.kind == kTurn) {
-        if (append && s_seq[tok] < 0) continue;
-        const long long z = append ? 0 : t / p.tokens;
-        dst += z * q.out_stride[0] + head[j] * q.out_stride[1] + (t - z * p.tokens) * q.out_stride[2];
-      } else {
-        if (s_page[tok] < 0) continue;
-        dst += s_page[tok] * q.out_stride[0] + (s_pos[tok] & (slots - 1)) * q.out_stride[1] + head[j] * q.out_stride[2];
-      }
-      if (k < q.turned) {
-        const int c1 = p.rope.interleaved ? 2 * k * V : k * V;
-        const int c2 = p.rope.interleaved ? c1 + V : c1 + half_dim;
-        const float2 *cs = turn + tok * half_dim + k * V;
-        T flat[2 * V];
+      for (int e = 0; e < V; ++e) cs[e] = turns ? turn[e * p.turned + k] : make_float2(1.f, 0.f);
+      // ---- the heads ----
+      const int c1 = turns ? (p.rope.interleaved ? 2 * k * V : k * V) : from + (k - turned) * V;
+      const int c2 = p.rope.interleaved ? c1 + V : c1 + half_dim;
+      const int step = static_cast<int>(p.slices) * beside;
+      for (int h0 = slice * beside; h0 < q.heads; h0 += step * kUnroll) {
+        Pack<T, V> a[kUnroll], b[kUnroll];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          flat[i] = a[j].x[i];
-          flat[V + i] = b[j].x[i];
-        }
-        if (p.rope.interleaved) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float x1 = rot_f32(flat[2 * i]), x2 = rot_f32(flat[2 * i + 1]);
-            flat[2 * i] = rot_from<T>(x1 * cs[i].x - x2 * cs[i].y);
-            flat[2 * i + 1] = rot_from<T>(x2 * cs[i].x + x1 * cs[i].y);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float x1 = rot_f32(flat[i]), x2 = rot_f32(flat[V + i]);
-            flat[i] = rot_from<T>(x1 * cs[i].x - x2 * cs[i].y);
-            flat[V + i] = rot_from<T>(x2 * cs[i].x + x1 * cs[i].y);
+        for (int u = 0; u < kUnroll; ++u) {
+          const int h = h0 + u * step + hl;
+          if (active && h < q.heads) {
+            const T *x = src + h * q.in_stride[1];
+            a[u] = *reinterpret_cast<const Pack<T, V> *>(x + c1);
+            if (turns) b[u] = *reinterpret_cast<const Pack<T, V> *>(x + c2);
           }
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          a[j].x[i] = flat[i];
-          b[j].x[i] = flat[V + i];
+        for (int u = 0; u < kUnroll; ++u) {
+          const int h = h0 + u * step + hl;
+          if (!(active && h < q.heads)) continue;
+          T *y = dst + h * dst_head;
+          if (turns) {
+            turn_pairs<T, V>(a[u], b[u], cs, p.rope.interleaved != 0);
+            *reinterpret_cast<Pack<T, V> *>(y + c2) = b[u];
+          }
+          *reinterpret_cast<Pack<T, V> *>(y + c1) = a[u];
         }
-        *reinterpret_cast<Pack<T, V> *>(dst + c1) = a[j];
-        *reinterpret_cast<Pack<T, V> *>(dst + c2) = b[j];
-      } else {
-        *reinterpret_cast<Pack<T, V> *>(dst + (q.turned ? p.rope.rotary_dim : 0) + (k - q.turned) * V) = a[j];
       }
     }
   }
