@@ -20,7 +20,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import backend as B
-from .rotary import Rope, _on, check  # noqa: F401  (check: part of this module's interface)
+from .rotary import Rope, _call, check  # noqa: F401  (check: part of this module's interface)
 
 _DTYPES = {torch.float16: B.TXD_F16, torch.bfloat16: B.TXD_BF16}
 MAX_LIST = 4096  # rows in one reserve
@@ -49,10 +49,6 @@ def _lib() -> ctypes.CDLL:
         lib.tx_paged_kernel_launches.restype = ctypes.c_uint64
         _lib_cache = lib
     return _lib_cache
-
-
-def _raise(lib, rc: int):
-    raise B.DotError(rc, lib.tx_paged_last_error().decode())
 
 
 def _invalid(text: str):
@@ -95,9 +91,9 @@ def _view(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor
 
 
 def _token_strides(x: torch.Tensor, name: str, tokens: int, head_dim: int, like: torch.Tensor) -> tuple[int, int]:
-    if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != head_dim or x.dtype != like.dtype or x.device != like.device:
+    shape, s = x.shape, x.stride()
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim or x.dtype != like.dtype or x.device != like.device:
         _invalid(f"{name} must be [tokens, heads, head_dim] = [{tokens}, *, {head_dim}] of the cache's type and device")
-    s = x.stride()
     if s[2] != 1 and head_dim > 1:
         _invalid(f"head_dim must be the contiguous dimension of {name}")
     return s[0], s[1]
@@ -132,7 +128,7 @@ def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages:
     if q is not None:
         qs, q_heads = _token_strides(q, "q", tokens, d, k_pages), q.shape[1]
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q)
         elif out.shape != q.shape or (tokens > 1 and out.stride(0) == 0) or (q_heads > 1 and out.stride(1) == 0):
             _invalid("out must have the shape of q and not be an expanded tensor")
         os_ = _token_strides(out, "out", tokens, d, k_pages)
@@ -142,10 +138,7 @@ def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages:
     if rope is not None and rope.rotary_dim > d:
         _invalid(f"rotary_dim {rope.rotary_dim} exceeds head_dim {d}")
     problem = _APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, *qs, *ks, *vs, *os_, tokens, q_heads)
-    with _on(k.device) as stream:
-        rc = lib.tx_paged_append(view, rope._packed if rope is not None else None, problem, stream)
-    if rc:
-        _raise(lib, rc)
+    _call(k.device, lib.tx_paged_append, view, rope._packed if rope is not None else None, problem)
     return out
 
 
@@ -177,19 +170,16 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     elif max_q is None:
         _invalid("cu_q needs max_q, a bound on the new tokens of one sequence")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or (tokens > 1 and out.stride(0) == 0) or (heads > 1 and out.stride(1) == 0):
         _invalid("out must have the shape of q and not be an expanded tensor")
     os_ = _token_strides(out, "out", tokens, d, k_pages)
     m = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_m else None
     problem = _ATTN.pack(q.data_ptr(), out.data_ptr(), m.data_ptr() if return_m else 0, qs[0], qs[1], os_[0], os_[1], tokens,
                          heads, max_q, int(causal), window, sm_scale)
-    with _on(device) as stream:
-        size = lib.tx_paged_attention_workspace(view, problem)
-        ws = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
-        rc = lib.tx_paged_attention(view, problem, ws.data_ptr() if ws is not None else None, size, stream)
-    if rc:
-        _raise(lib, rc)
+    size = lib.tx_paged_attention_workspace(view, problem)
+    ws = q.new_empty((size + 1) // 2)  # 16-bit values
+    _call(device, lib.tx_paged_attention, view, problem, ws.data_ptr(), size)
     return (out, m) if return_m else out
 
 
@@ -240,27 +230,21 @@ class PagedCache:
             _invalid(f"{name} must be an int32 vector{f' of {n}' if n is not None else ''} on the device of the cache")
         return x if x.is_contiguous() else x.contiguous()
 
-    def _workspace(self, lib, n: int) -> torch.Tensor:
-        return torch.empty(lib.tx_pages_workspace(self._state, n), dtype=torch.uint8, device=self.k.device)
+    def _workspace(self, lib, rows: torch.Tensor) -> torch.Tensor:
+        return rows.new_empty((lib.tx_pages_workspace(self._state, rows.shape[0]) + 3) // 4)
 
     def free(self, rows: torch.Tensor) -> None:
         """Give the pages of the listed rows back (those that no other row holds become free) and empty the rows."""
         lib, rows = _lib(), self._list(rows, "rows")
-        with _on(self.k.device) as stream:
-            rc = lib.tx_pages_free(self._state, rows.data_ptr(), rows.shape[0], stream)
-        if rc:
-            _raise(lib, rc)
+        _call(rows.device, lib.tx_pages_free, self._state, rows.data_ptr(), rows.shape[0])
 
     def fork(self, dst: torch.Tensor, src: torch.Tensor) -> None:
         """Row dst[i] becomes what row src[i] was before the call, sharing its pages. Rows may be both (the reordering of a
         beam search); what a destination held is given back; of a destination listed twice the last one holds."""
         lib, dst = _lib(), self._list(dst, "dst")
         src = self._list(src, "src", dst.shape[0])
-        with _on(self.k.device) as stream:
-            ws = self._workspace(lib, dst.shape[0])
-            rc = lib.tx_pages_fork(self._state, dst.data_ptr(), src.data_ptr(), dst.shape[0], ws.data_ptr(), stream)
-        if rc:
-            _raise(lib, rc)
+        ws = self._workspace(lib, dst)
+        _call(dst.device, lib.tx_pages_fork, self._state, dst.data_ptr(), src.data_ptr(), dst.shape[0], ws.data_ptr())
 
     def reserve(self, rows: torch.Tensor, counts: torch.Tensor) -> None:
         """Make room for counts[i] more tokens in row rows[i] and add them to its length, before they are appended. New pages
@@ -268,22 +252,16 @@ class PagedCache:
         of the listed rows that alone share one, the last keeps it."""
         lib, rows = _lib(), self._list(rows, "rows")
         counts = self._list(counts, "counts", rows.shape[0])
-        with _on(self.k.device) as stream:
-            ws = self._workspace(lib, rows.shape[0])
-            rc = lib.tx_pages_reserve(self._state, rows.data_ptr(), counts.data_ptr(), rows.shape[0], ws.data_ptr(), stream)
-        if rc:
-            _raise(lib, rc)
+        ws = self._workspace(lib, rows)
+        _call(rows.device, lib.tx_pages_reserve, self._state, rows.data_ptr(), counts.data_ptr(), rows.shape[0], ws.data_ptr())
 
     def compact(self) -> None:
         """Move pages (all layers) so that the used ones are the lowest, the fewest that do it; the table follows."""
         lib = _lib()
         if not self.k.is_cuda:
             _not_cuda(self.k)
-        with _on(self.k.device) as stream:
-            ws = self._workspace(lib, 0)
-            rc = lib.tx_pages_compact(self._state, ws.data_ptr(), stream)
-        if rc:
-            _raise(lib, rc)
+        ws = self.refs.new_empty((lib.tx_pages_workspace(self._state, 0) + 3) // 4)
+        _call(self.k.device, lib.tx_pages_compact, self._state, ws.data_ptr())
 
     def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
         """Copy the contents of pages src[i] to dst[i] in every layer. Host lists; no page may be a destination twice, or
@@ -297,7 +275,4 @@ class PagedCache:
         for x in (*src, *dst):
             if not 0 <= int(x) < pages:
                 _invalid(f"page {x} is outside the {pages} pages")
-        with _on(self.k.device) as stream:
-            rc = lib.tx_pages_copy(self._state, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n, stream)
-        if rc:
-            _raise(lib, rc)
+        _call(self.k.device, lib.tx_pages_copy, self._state, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n)

@@ -24,6 +24,13 @@ _DTYPES = {torch.float16: B.TXD_F16, torch.bfloat16: B.TXD_BF16, torch.float32: 
 # 1 / (2 pi) to 100 binary digits: a product with an exact double gives all 64 bits of a turn's fraction
 _INV_2PI = Fraction(201752859139730814931732094791, 1 << 100)
 
+
+def _turns(w: float) -> int:
+    """w / (2 pi) as a 64-bit fraction of a turn, rounded to nearest."""
+    n, d = w.as_integer_ratio()
+    d <<= 100 - 64
+    return ((2 * n * _INV_2PI.numerator + d) // (2 * d)) & 0xFFFFFFFFFFFFFFFF
+
 _lib_cache = None
 
 
@@ -40,10 +47,6 @@ def _lib() -> ctypes.CDLL:
         lib.tx_paged_check.restype = ctypes.c_int
         _lib_cache = lib
     return _lib_cache
-
-
-def _raise(lib, rc: int):
-    raise B.DotError(rc, lib.tx_paged_last_error().decode())
 
 
 def kernel_launches() -> int:
@@ -98,7 +101,7 @@ class Rope:
         if magnitude is None:
             magnitude = 0.1 * math.log(factor) + 1.0 if scaling == "parts" else 1.0
         self.rotary_dim, self.interleaved, self.frequencies, self.magnitude = rotary_dim, interleaved, tuple(freq), magnitude
-        turns = [round(Fraction(w) * _INV_2PI * (1 << 64)) & 0xFFFFFFFFFFFFFFFF for w in freq]
+        turns = [_turns(w) for w in freq]
         self._packed = struct.pack(f"iifi{MAX_PAIRS}Q", rotary_dim, int(interleaved), magnitude, 0,
                                    *(turns + [0] * (MAX_PAIRS - pairs)))
 
@@ -171,30 +174,22 @@ def rotary_forward(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.
         parts, second = 2, _part(k, out_k)
     packed = _HEAD.pack(z, n, d, dtype, int(inverse), int(positions.dtype == torch.int64), pos_stride[0], pos_stride[1],
                         parts, 0) + _part(q, out_q) + second
-    with _on(q.device) as stream:
-        rc = lib.tx_rotary(rope._packed, packed, positions.data_ptr(), stream)
-    if rc:
-        _raise(lib, rc)
+    _call(q.device, lib.tx_rotary, rope._packed, packed, positions.data_ptr())
     return out_q, (out_k if k is not None else None)
 
 
-class _on:
-    """The current stream's handle of a device, which is made the current device meanwhile."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _call(device: torch.device, function, *args) -> None:
+    """One C entry point on the current stream of a device (made the current device meanwhile); raises if it fails. The
+    stream is the entry point's last argument."""
+    index = device.index
+    before = torch.cuda.current_device()
+    if before == index:
+        rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        raise B.DotError(rc, _lib().tx_paged_last_error().decode())
 
 
 class _Rotary(torch.autograd.Function):
@@ -209,11 +204,16 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, gq, gk):
         (positions,) = ctx.saved_tensors
         rope, inverse = ctx.rope, not ctx.inverse
-        # the gradient of a turn is the turn backwards, which autograd may differentiate again
-        if gq is None and gk is not None:
-            gk = _Rotary.apply(gk, None, positions, rope, inverse)[0]
-        elif gq is not None:
-            gq, gk = _Rotary.apply(gq, gk, positions, rope, inverse)
+        # the gradient of a turn is the turn backwards; where it is to be differentiated again, as a function itself
+        again = torch.is_grad_enabled()
+
+        def turn(a, b):
+            return _Rotary.apply(a, b, positions, rope, inverse) if again else rotary_forward(a, b, positions, rope, inverse=inverse)
+
+        if gq is not None:
+            gq, gk = turn(gq, gk)
+        elif gk is not None:
+            gk = turn(gk, None)[0]
         return gq, gk, None, None, None
 
 
@@ -228,11 +228,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
 def check(device=None) -> None:
     """Synchronise the current stream and raise for what the rotary, append, paged attention and page kernels found wrong
     on the device since the last check."""
-    lib = _lib()
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    dev = torch.device("cuda") if device is None else torch.device(device)
     if dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
-    with _on(dev) as stream:
-        rc = lib.tx_paged_check(stream)
-    if rc:
-        _raise(lib, rc)
+    _call(dev, _lib().tx_paged_check)
