@@ -47,15 +47,15 @@ int encode_pool(CUtensorMap *map, const void *ptr, const tx_paged_view &c, const
   return TXD_OK;
 }
 
-// Queries as {head_dim, heads, tokens}; a box is the heads of one key head of a sub-tile's tokens.
+// Queries as {head_dim, heads, tokens}; a box is the heads of one key head of a sub-tile's tokens, every `every`-th one.
 int encode_queries(CUtensorMap *map, const void *ptr, const tx_paged_view &c, const int64_t *stride, int heads, int tokens,
-                   int group, int sub_tokens) {
+                   int group, int sub_tokens, int every) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return fail(TXD_ERR_NO_DEVICE, "cuTensorMapEncodeTiled is not available from the CUDA driver");
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride[1]) * 2, static_cast<cuuint64_t>(stride[0]) * 2};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(sub_tokens)};
-  const cuuint32_t estr[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(sub_tokens * every)};
+  const cuuint32_t estr[3] = {1, 1, static_cast<cuuint32_t>(every)};
   const CUresult r = enc(map, c.dtype == TXD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                          const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -207,14 +207,20 @@ uint32_t mma_idesc(bool bf16, bool b_mn_major, int n) {
   return 1u << 4 | type << 7 | type << 10 | (b_mn_major ? 1u : 0u) << 16 | static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
 }
 
+template <typename T, int D>
+int launch_join_d(const Plan &plan, const JoinParams &j, cudaStream_t s) {
+  const int units = (plan.rows + 31) / 32 * (D / 16);  // warps of a tile, or blocks where few rows are joined
+  if (plan.rows <= 64) TXP_CUDA(launch(paged_join_kernel<T, D, true>, dim3(j.ctas - 1, units), dim3(256), 0, s, j));
+  else TXP_CUDA(launch(paged_join_kernel<T, D, false>, dim3(j.ctas - 1, (units + 7) / 8), dim3(256), 0, s, j));
+  return TXD_OK;
+}
+
 template <typename T>
 int launch_join(const Plan &plan, const JoinParams &j, cudaStream_t s) {
   if (j.ctas < 2) return TXD_OK;
-  const dim3 grid(j.ctas - 1, (plan.rows + 7) / 8);
-  if (plan.kernel_d == 64) TXP_CUDA(launch(paged_join_kernel<T, 64>, grid, dim3(256), 0, s, j));
-  else if (plan.kernel_d == 128) TXP_CUDA(launch(paged_join_kernel<T, 128>, grid, dim3(256), 0, s, j));
-  else TXP_CUDA(launch(paged_join_kernel<T, 256>, grid, dim3(256), 0, s, j));
-  return TXD_OK;
+  if (plan.kernel_d == 64) return launch_join_d<T, 64>(plan, j, s);
+  if (plan.kernel_d == 128) return launch_join_d<T, 128>(plan, j, s);
+  return launch_join_d<T, 256>(plan, j, s);
 }
 
 unsigned long long wait_limit() {
@@ -278,6 +284,7 @@ int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_problem *
   sched.tile_cost = 2;
   sched.min_part = 2;
   sched.min_share = 4;
+  sched.waves = kMaxWaves;
   sched.status = status;
 
   if (plan.tiled) {
@@ -287,7 +294,7 @@ int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_problem *
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   const bool bf16 = c.dtype == TXD_BF16;
   int4 *borders = reinterpret_cast<int4 *>(ws);
-  float *part = reinterpret_cast<float *>(ws + plan.borders_bytes);
+  float4 *part = reinterpret_cast<float4 *>(ws + plan.borders_bytes);
   float2 *ml = reinterpret_cast<float2 *>(ws + plan.borders_bytes + plan.part_bytes);
   const float qk_scale = pr->sm_scale * 1.44269504f;  // 1 / ln 2
   int32_t inject_stall = 0;
@@ -316,7 +323,8 @@ int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_problem *
     const int box_rows = c.page_size < 128 ? c.page_size : 128;
     prm.sub_tokens = 128 / plan.group;
     prm.part_rows = plan.rows;
-    if ((rc = encode_queries(&prm.tmap_q, pr->q, c, q_stride, pr->q_heads, pr->tokens, plan.group, prm.sub_tokens))) return rc;
+    for (int i = 0; i < 2; ++i)
+      if ((rc = encode_queries(i ? &prm.tmap_q2 : &prm.tmap_q, pr->q, c, q_stride, pr->q_heads, pr->tokens, plan.group, prm.sub_tokens, i + 1))) return rc;
     if ((rc = encode_pool(&prm.tmap_k, c.k, c, c.k_stride, box_rows, 1))) return rc;
     if ((rc = encode_pool(&prm.tmap_v, c.v, c, c.v_stride, box_rows, 1))) return rc;
     fill(prm, box_rows);

@@ -32,7 +32,7 @@ struct RowParams {
   const int32_t *table;
   long long table_stride;
   int4 *borders;
-  float *part;
+  float4 *part;
   float2 *ml;
   unsigned long long wait_limit_ns;
   float qk_scale;  // sm_scale * log2(e)
@@ -110,8 +110,8 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
     tma_prefetch_desc(&p.tmap_v);
   }
   grid_dep_wait();
-  const bool work = find_stretch<kThreads>(p.s, &sched, p.borders);  // syncs the CTA
-  if (!work) return;
+  find_work<kThreads, false>(p.s, &sched, p.borders, nullptr);
+  __syncthreads();
 
   AbortCtl ac;
   ac.flag = &abort_flag;
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
     bool ok = true;
     const int boxes = kRowBlock >> p.box_shift;           // copies of a tensor per block
     const uint32_t box_bytes = (128u << p.box_shift) * kGroups;
-    for (bool more = w.start(p.s, &sched); more && ok; more = w.next(p.s)) {
+    for (bool more = w.start(p.s, &sched); more && ok; more = w.next(p.s, &sched)) {
       const int32_t *row = p.table + w.at.b * p.table_stride;
       const int first_page = w.t.lo >> p.page_shift, last_page = (w.t.hi - 1) >> p.page_shift;
       int window = -1, page_reg = 0;  // 32 entries of the page table, one a lane
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
     const uint32_t k_row = ((lane >> 4) * 8 + x7) * 128u, k_chunk = (lane >> 3) & 1;
     const uint32_t v_row = (((lane >> 3) & 1) * 8 + x7) * 128u, v_chunk = lane >> 4;
 
-    for (bool more = w.start(p.s, &sched); more; more = w.next(p.s)) {
+    for (bool more = w.start(p.s, &sched); more; more = w.next(p.s, &sched)) {
       const int rows = (w.t.t1 - w.t.t0) * p.s.group;
       // ---- Q: the A fragments of this warp's 16 rows, straight from memory ----
       uint32_t qf[D / 16][4];
@@ -381,7 +381,9 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
           asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
         }
         for (int idx = threadIdx.x; idx < MT * 16 * (kJoinCols / 4); idx += kConsumers * 32) {
-          const int r = idx / (kJoinCols / 4), c = (idx % (kJoinCols / 4)) * 4, col = round * kJoinCols + c;
+          // neighbouring threads take neighbouring columns of the output, or neighbouring rows of a partial result
+          const int r = whole ? idx / (kJoinCols / 4) : idx % (MT * 16);
+          const int c = (whole ? idx % (kJoinCols / 4) : idx / (MT * 16)) * 4, col = round * kJoinCols + c;
           if (r >= rows) continue;
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
           float top = -INFINITY, sum = 0.f;
@@ -411,9 +413,8 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
             }
             if (p.m_out && col == 0) p.m_out[static_cast<long long>(tok) * p.heads + head] = sum > 0.f ? top + log2f(sum) : -INFINITY;
           } else {
-            const long long at = (static_cast<long long>(blockIdx.x) * 2 + w.slot()) * (MT * 16) + r;
-            *reinterpret_cast<float4 *>(p.part + at * D + col) = x;
-            if (col == 0) p.ml[at] = make_float2(top, sum);
+            p.part[(w.slot() * (D / 4) + col / 4) * (MT * 16) + r] = x;
+            if (col == 0) p.ml[w.slot() * (MT * 16) + r] = make_float2(top, sum);
           }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");

@@ -2,11 +2,13 @@
 //
 // The work is a line of tiles, in order of sequence, key head and query tile (T new tokens with the G query heads of one key
 // head: T * G rows); a tile is as long as the KV blocks that its rows see, plus a constant for what a tile costs besides.
-// CTA c of n takes the stretch [total * c / n, total * (c + 1) / n) of that line, so ragged batches, causal triangles and
-// a single sequence over a long cache are all shared evenly. A tile that a border cuts is attended to in parts: each part leaves
-// its unnormalised output, maximum and sum in the workspace (at most two parts of a CTA are not whole tiles: its first and
-// its last), and a second kernel joins them in order. Nothing waits for another CTA, nothing is counted with atomics, and
-// the order of every sum depends on the lengths alone.
+// Few long tiles (a single sequence over a long cache, a batch of single tokens): the line is cut into n equal stretches, one
+// a CTA. Many tiles: the first F * n are dealt out whole, wave by wave, every second wave in reverse, so that the CTAs that
+// run at the same time are at neighbouring tiles and share their keys and values through L2 (all CTAs on contiguous
+// stretches took 4.74 ms for 32 heads of 16384 tokens of 128, this 3.92: every head's keys were in use at once); the
+// rest of the line is cut so that all CTAs come to the same length. Either way a CTA has at most two parts of tiles:
+// those leave their unnormalised output, maximum and sum in the workspace, and a second kernel joins them in order.
+// Nothing waits for another CTA, nothing is counted with atomics, and the order of every sum depends on the lengths alone.
 //
 // Every CTA finds its borders itself, from the lengths: one pass over the batch for the total and one for the places.
 #pragma once
@@ -30,7 +32,8 @@ struct Sched {
   int32_t block_shift;         // log2 of the KV block
   int32_t tile_cost;           // of a tile besides its blocks, in blocks
   int32_t min_part;            // no part is shorter, in blocks
-  int32_t min_share;           // no CTA's share is shorter (fewer CTAs work then)
+  int32_t min_share;           // no stretch is shorter (there are fewer then)
+  int32_t waves;               // at most so many waves of whole tiles
   uint32_t *status;
 };
 
@@ -100,10 +103,11 @@ __device__ __forceinline__ void next_tile(const Sched &s, Cut &c, SeqInfo &q) {
 __device__ __forceinline__ bool same_tile(const Cut &a, const Cut &b) { return a.b == b.b && a.h == b.h && a.i == b.i; }
 
 // The place at distance r along the tiles of sequence b, moved to a tile's start where a part would be too short.
-__device__ __forceinline__ Cut resolve(const Sched &s, int b, long long r, long long per_head) {
+__device__ __forceinline__ Cut resolve(const Sched &s, int b, long long distance, long long per_head) {
   SeqInfo q = seq_info(s, b);
-  Cut c = {b, static_cast<int>(r / per_head), 0, 0};
-  r -= c.h * per_head;
+  const int h = static_cast<int>(distance / per_head);
+  long long r = distance - h * per_head;
+  Cut c = {b, h, 0, 0};
   TileInfo t = tile_info(s, q, 0);
   while (r >= t.n + s.tile_cost) {
     r -= t.n + s.tile_cost;
@@ -115,93 +119,185 @@ __device__ __forceinline__ Cut resolve(const Sched &s, int b, long long r, long 
   return c;
 }
 
-template <int kThreads>
-__device__ __forceinline__ long long block_sum_scan(long long x, long long *total, long long *sums) {
+// Exclusive prefix sums over a block, of one or two values a thread at once; their totals for everyone.
+template <int kThreads, int kValues>
+__device__ __forceinline__ void block_scan(long long (&x)[kValues], long long (&total)[kValues], long long *sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long sum = x;
+  constexpr int kWarps = kThreads / 32;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, sum, d);
-    if (lane >= d) sum += y;
-  }
-  if (lane == 31) sums[warp] = sum;
-  __syncthreads();
-  long long before = 0, all = 0;
+  for (int v = 0; v < kValues; ++v) {
+    long long sum = x[v];
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += sums[w];
-    all += sums[w];
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += y;
+    }
+    if (lane == 31) sums[v * 32 + warp] = sum;
+    x[v] = sum - x[v];
   }
-  *total = all;
   __syncthreads();
-  return before + sum - x;
+#pragma unroll
+  for (int v = 0; v < kValues; ++v) {
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const long long y = sums[v * 32 + w];
+      if (w < warp) before += y;
+      all += y;
+    }
+    x[v] += before;
+    total[v] = all;
+  }
+  __syncthreads();
 }
 
+constexpr int kMaxWaves = 16;
+
 struct SchedSmem {
-  long long sums[32];
-  Cut cut[2];
+  long long sums[64];
+  long long x[2];               // this CTA's stretch
+  int waves;
+  Cut cut[kMaxWaves + 2];       // its whole tiles, then the ends of its stretch
 };
 
-// For all threads of a CTA: its stretch goes to sm->cut[0], sm->cut[1]; false when there is nothing for it. Its first
-// border is also written to `borders` (b = -1 where no tile is cut), for the joining kernel.
-template <int kThreads>
-__device__ __forceinline__ bool find_stretch(const Sched &s, SchedSmem *sm, int4 *borders) {
-  const int cta = blockIdx.x;
+// What the dealing-out of whole tiles needs of every sequence; one entry a thread.
+struct SeqTable {
+  int *tiles_before, *q, *kv;   // tiles of the sequences before; the sequence's lengths
+};
+
+__device__ __forceinline__ Cut tile_at(const Sched &s, const SeqTable &tab, int index) {
+  int lo = 0, hi = s.batch - 1;  // the last sequence whose tiles start at or before the index
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (tab.tiles_before[mid] <= index) lo = mid;
+    else hi = mid - 1;
+  }
+  const int per_head = (tab.q[lo] + s.tile_tokens - 1) / s.tile_tokens;
+  const int r = index - tab.tiles_before[lo], h = r / per_head;
+  return Cut{lo, h, r - h * per_head, 0};
+}
+
+__device__ __forceinline__ int tile_length(const Sched &s, const SeqTable &tab, const Cut &c) {
+  return tile_info(s, SeqInfo{0, tab.q[c.b], tab.kv[c.b]}, c.i).n + s.tile_cost;
+}
+
+// For all threads of a CTA: its work goes to *sm, and the first border of its stretch also to `borders` (b = -1 where no
+// tile is cut; block -1 where the stretch is empty), for the joining kernel. kWaves: whole tiles are dealt out (`scratch`:
+// 3 * kThreads ints of shared memory).
+template <int kThreads, bool kWaves>
+__device__ __forceinline__ void find_work(const Sched &s, SchedSmem *sm, int4 *borders, int *scratch) {
+  const int cta = blockIdx.x, n = gridDim.x, tid = threadIdx.x;
   const bool one_pass = s.batch <= kThreads;
-  long long mine = 0, per_head = 0, total;
-  for (int b = threadIdx.x; b < s.batch; b += kThreads) {
-    const SeqInfo q = seq_info(s, b);
+  long long mine = 0, per_head = 0;
+  SeqInfo q = {0, 0, 0};
+  for (int b = tid; b < s.batch; b += kThreads) {
+    q = seq_info(s, b);
     if (cta == 0 && s.kv_lens[b] > s.max_kv) atomicOr(s.status, kNoRoomInRow);
     per_head = head_cost(s, q);
     mine += per_head * s.kv_heads;
   }
-  const long long before = block_sum_scan<kThreads>(mine, &total, sm->sums);
-  const long long most = total / s.min_share;
-  const int n = most < static_cast<int>(gridDim.x) ? max(static_cast<int>(most), 1) : gridDim.x;
-  const long long x0 = total * cta / n, x1 = total * (cta + 1) / n;
-  if (threadIdx.x == 0) sm->cut[0] = sm->cut[1] = Cut{s.batch, 0, 0, 0};
+  if (tid < kMaxWaves + 2) sm->cut[tid] = Cut{s.batch, 0, 0, 0};
+  if (tid == 0) sm->waves = kMaxWaves, sm->x[0] = sm->x[1] = -1;
+  long long before[2] = {mine, tid < s.batch ? static_cast<long long>(tiles_of(s, q)) * s.kv_heads : 0}, totals[2];
+  block_scan<kThreads, 2>(before, totals, sm->sums);
+  const long long total = totals[0];
+  long long skipped = 0;  // length of what is dealt out whole
+  int waves = 0;
+  long long dealt[2] = {0, 0}, dealt_all[2] = {0, 1};  // thread c: CTA c's whole tiles, and what is left for its stretch
+  if (kWaves && one_pass && n <= kThreads && totals[1] >= n && totals[1] < INT32_MAX) {
+    const SeqTable tab = {scratch, scratch + kThreads, scratch + 2 * kThreads};
+    tab.tiles_before[tid] = static_cast<int>(before[1]);
+    tab.q[tid] = q.q;
+    tab.kv[tid] = q.kv;
+    __syncthreads();
+    const int most = min(static_cast<int>(totals[1]) / n, s.waves);
+    const long long target = total / n;
+    auto tile_of = [&](int f) { return tile_at(s, tab, f * n + ((f & 1) ? n - 1 - tid : tid)); };
+    // only as many waves as no CTA's whole tiles alone are more than its share of the work
+    int fit = 0;
+    if (tid < n) {
+      for (; fit < most; ++fit) {
+        const Cut c = tile_of(fit);
+        const int length = tile_length(s, tab, c);
+        if (dealt[0] + length > target + s.tile_cost) break;
+        dealt[0] += length;
+        if (tid == cta) sm->cut[fit] = c;
+      }
+      atomicMin(&sm->waves, fit);
+    }
+    __syncthreads();
+    waves = sm->waves;
+    for (int f = waves; f < fit; ++f) dealt[0] -= tile_length(s, tab, tile_of(f));
+    if (tid < n) dealt[1] = max(target + 1 - dealt[0], 0ll);
+    block_scan<kThreads, 2>(dealt, dealt_all, sm->sums);
+    skipped = dealt_all[0];
+    if (tid == cta)
+      for (int f = waves; f < fit; ++f) sm->cut[f] = Cut{s.batch, 0, 0, 0};
+  }
+  // ---- the rest of the line ----
+  const long long rest = total - skipped;
+  const int parts = rest < static_cast<long long>(s.min_share) * n ? max(static_cast<int>(rest) / s.min_share, 1) : n;
+  if (waves > 0 && parts == n) {
+    // (in double: the product of two lengths may pass 2^63, and rounding keeps the borders' order)
+    if (tid == cta || tid == cta + 1)
+      sm->x[tid - cta] = skipped + static_cast<long long>(static_cast<double>(rest) * (static_cast<double>(dealt[1]) / static_cast<double>(dealt_all[1])));
+    if (tid == cta && cta == n - 1) sm->x[1] = total;
+  } else if (tid < 2 && cta < parts && rest > 0) {
+    sm->x[tid] = skipped + rest * (cta + tid) / parts;
+  }
+  if (tid == 0) sm->waves = waves;
   __syncthreads();
-  if (cta < n) {
-    if (one_pass) {
-      if (threadIdx.x < s.batch) {
-        if (x0 >= before && x0 < before + mine) sm->cut[0] = resolve(s, threadIdx.x, x0 - before, per_head);
-        if (x1 >= before && x1 < before + mine) sm->cut[1] = resolve(s, threadIdx.x, x1 - before, per_head);
-      }
-    } else {
-      long long carry = 0;
-      for (int base = 0; base < s.batch; base += kThreads) {
-        const int b = base + threadIdx.x;
-        long long chunk;
-        per_head = b < s.batch ? head_cost(s, seq_info(s, b)) : 0;
-        mine = per_head * s.kv_heads;
-        const long long at = carry + block_sum_scan<kThreads>(mine, &chunk, sm->sums);
-        if (x0 >= at && x0 < at + mine) sm->cut[0] = resolve(s, b, x0 - at, per_head);
-        if (x1 >= at && x1 < at + mine) sm->cut[1] = resolve(s, b, x1 - at, per_head);
-        carry += chunk;
-      }
+  const long long x0 = sm->x[0], x1 = sm->x[1];
+  auto place = [&](int b, long long at, long long cost, long long head) {
+    if (x0 >= at && x0 < at + cost) sm->cut[waves] = resolve(s, b, x0 - at, head);
+    if (x1 >= at && x1 < at + cost) sm->cut[waves + 1] = resolve(s, b, x1 - at, head);
+  };
+  if (one_pass) {
+    if (mine > 0) place(tid, before[0], mine, per_head);
+  } else {
+    long long carry = 0;
+    for (int base = 0; base < s.batch; base += kThreads) {
+      const int b = base + tid;
+      per_head = b < s.batch ? head_cost(s, seq_info(s, b)) : 0;
+      mine = per_head * s.kv_heads;
+      long long at[1] = {mine}, chunk[1];
+      block_scan<kThreads, 1>(at, chunk, sm->sums);
+      if (mine > 0) place(b, carry + at[0], mine, per_head);
+      carry += chunk[0];
     }
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const Cut c = sm->cut[0];
-    borders[cta] = cta < n && c.blk > 0 ? make_int4(c.b, c.h, c.i, c.blk) : make_int4(-1, 0, 0, 0);
+  if (tid == 0) {
+    const Cut c = sm->cut[waves], e = sm->cut[waves + 1];
+    const bool empty = same_tile(c, e) && c.blk == e.blk;  // its whole tiles were as long as its share
+    borders[cta] = x0 >= 0 && c.blk > 0 ? make_int4(c.b, c.h, c.i, empty ? -1 : c.blk) : make_int4(-1, 0, 0, 0);
   }
-  const Cut a = sm->cut[0], b = sm->cut[1];
-  return cta < n && !(same_tile(a, b) && a.blk == b.blk);
 }
 
-// A stretch walked tile by tile (every role warp walks it by itself).
+// A CTA's work walked tile by tile (every role warp walks it by itself).
 struct Walk {
   Cut at, end;
   SeqInfo q;
   TileInfo t;
-  int from, to;  // blocks of the current tile in this stretch, relative to its first
+  int from, to;  // blocks of the current tile in this CTA's work, relative to its first
+  int wave;
   __device__ __forceinline__ bool start(const Sched &s, const SchedSmem *sm) {
-    at = sm->cut[0];
-    end = sm->cut[1];
-    if (at.b >= s.batch || (same_tile(at, end) && at.blk == end.blk)) return false;
+    wave = -1;
+    return open(s, sm);
+  }
+  // the next whole tile, or the stretch
+  __device__ __forceinline__ bool open(const Sched &s, const SchedSmem *sm) {
+    if (++wave > sm->waves) return false;
+    at = sm->cut[wave];
+    if (at.b >= s.batch) return false;
+    if (wave == sm->waves) {
+      end = sm->cut[wave + 1];
+      if (same_tile(at, end) && at.blk == end.blk) return false;
+    }
+    else end = Cut{s.batch, 0, 0, 0};
     q = seq_info(s, at.b);
     load(s);
+    if (wave < sm->waves) end = Cut{at.b, at.h, at.i, to};
     return true;
   }
   __device__ __forceinline__ void load(const Sched &s) {
@@ -209,22 +305,23 @@ struct Walk {
     from = at.blk;
     to = same_tile(at, end) ? end.blk : t.n;
   }
-  __device__ __forceinline__ bool next(const Sched &s) {
-    if (same_tile(at, end)) return false;
+  __device__ __forceinline__ bool next(const Sched &s, const SchedSmem *sm) {
+    if (same_tile(at, end)) return open(s, sm);
     next_tile(s, at, q);
-    if (at.b >= s.batch || (same_tile(at, end) && end.blk == 0)) return false;
+    if (at.b >= s.batch || (same_tile(at, end) && end.blk == 0)) return open(s, sm);
     load(s);
     return true;
   }
   __device__ __forceinline__ bool whole() const { return from == 0 && to == t.n; }
-  __device__ __forceinline__ int slot() const { return from > 0 ? 0 : 1; }  // of this CTA's two partial results
+  // which of the partial results: a CTA has two, for the tile that its stretch begins in and the one that it ends in
+  __device__ __forceinline__ long long slot() const { return static_cast<long long>(blockIdx.x) * 2 + (from > 0 ? 0 : 1); }
 };
 
 // ---- joining the parts of cut tiles --------------------------------------------------------------------------------
 struct JoinParams {
   Sched s;
   const int4 *borders;  // [ctas]
-  const float *part;    // [ctas][2][rows][D], then
+  const float4 *part;   // [ctas][2][D / 4][rows]: four columns of a row together, rows next to each other
   const float2 *ml;     // [ctas][2][rows]: maximum (log2 units) and sum
   void *out;
   float *m_out;
@@ -232,22 +329,68 @@ struct JoinParams {
   int32_t ctas, rows, heads, head_dim;
 };
 
-// One warp joins one row: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. The parts of a tile are those of consecutive
-// CTAs; the block of a tile's first border does the tile. Bound by latency when there are few rows and by reading the
-// parts when there are many (L2 holds them).
-template <typename T, int D>
+// The joined value of a row: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, part by part.
+struct Joined {
+  float acc[16], top, sum;
+};
+
+template <int D>
+__device__ __forceinline__ Joined join_parts(const JoinParams &p, int c, int first, int step, int parts, int row, int col) {
+  Joined j;
+  j.top = -INFINITY;
+  j.sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) j.acc[e] = 0.f;
+  auto slot = [&](int i) { return static_cast<long long>(c - 1 + i) * 2 + (i == 0 ? 1 : 0); };
+  auto there = [&](int i) { return i == 0 || p.borders[c - 1 + i].w > 0; };  // an empty stretch has left nothing
+#pragma unroll 4
+  for (int i = first; i < parts; i += step)
+    if (there(i)) j.top = fmaxf(j.top, p.ml[slot(i) * p.rows + row].x);
+  const float ref = j.top == -INFINITY ? 0.f : j.top;
+#pragma unroll 2
+  for (int i = first; i < parts; i += step) {
+    if (!there(i)) continue;
+    const float2 ml = p.ml[slot(i) * p.rows + row];
+    const float4 *o = p.part + (slot(i) * (D / 4) + col / 4) * p.rows + row;
+    float4 x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = o[static_cast<long long>(e) * p.rows];
+    if (ml.x != -INFINITY) {  // a part that saw nothing has left no output
+      const float w = fast_exp2(ml.x - ref);
+      j.sum += w * ml.y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        j.acc[4 * e] += w * x[e].x;
+        j.acc[4 * e + 1] += w * x[e].y;
+        j.acc[4 * e + 2] += w * x[e].z;
+        j.acc[4 * e + 3] += w * x[e].w;
+      }
+    }
+  }
+  return j;
+}
+
+// The parts of a tile are those of consecutive CTAs; the blocks of a tile's first border do the tile. A thread joins 16
+// columns of one row (32 bytes of output, a whole sector), a warp's threads are 32 rows, which the parts are laid out for.
+// kFewRows (single tokens: up to a few dozen parts, 16 to 64 rows): the 8 warps of a block share a tile's parts, because
+// one thread after another part's loads is what takes the time there (2 x 131071 tokens: 112 us with a thread for all
+// parts, 98); else (256 rows, two or three parts) a warp does all of them, bound by reading them.
+template <typename T, int D, bool kFewRows>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ JoinParams p) {
-  constexpr int kVec = D / 32;  // columns of a lane
+  constexpr int kColGroups = D / 16;
+  __shared__ float s_acc[kFewRows ? 8 : 1][18][32];
   grid_dep_wait();
-  const int c = static_cast<int>(blockIdx.x) + 1, lane = threadIdx.x & 31;
+  const int c = static_cast<int>(blockIdx.x) + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int4 cut = p.borders[c], prev = p.borders[c - 1];
   if (cut.x < 0 || (prev.x == cut.x && prev.y == cut.y && prev.z == cut.z)) return;
   const SeqInfo q = seq_info(p.s, cut.x);
   const int t0 = cut.z * p.s.tile_tokens, t1 = min(t0 + p.s.tile_tokens, q.q);
-  const int row = static_cast<int>(blockIdx.y) * 8 + static_cast<int>(threadIdx.x >> 5);
-  if (row >= (t1 - t0) * p.s.group) return;
+  const int rows = (t1 - t0) * p.s.group;
+  const int unit = kFewRows ? blockIdx.y : blockIdx.y * 8 + warp;
+  const int row = unit / kColGroups * 32 + lane, col = unit % kColGroups * 16;
+  if (unit / kColGroups * 32 >= rows || col >= p.head_dim) return;  // for a whole warp, and block where they share
   int parts = 2;  // of CTAs c - 1 and c, and of those behind whose border lies in the tile as well
-  for (bool more = true; more; ) {
+  for (bool more = true; more;) {
     const int k = c + parts - 1 + lane;
     int4 x = make_int4(-1, 0, 0, 0);
     if (k < p.ctas) x = p.borders[k];
@@ -256,43 +399,43 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     parts += run;
     more = run == 32;
   }
-  auto place = [&](int i) { return (static_cast<long long>(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row; };
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.ml[place(i)].x);
+  Joined j;
+  if (kFewRows) {
+    if (row < rows) {
+      j = join_parts<D>(p, c, warp, 8, parts, row, col);
 #pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  const float ref = top == -INFINITY ? 0.f : top;
-  float acc[kVec], sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) acc[e] = 0.f;
-  for (int base = 0; base < parts; base += 32) {
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (base + lane < parts) ml = p.ml[place(base + lane)];
-    const float mine = fast_exp2(ml.x - ref);
-    const int count = min(parts - base, 32);
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-      const float w = __shfl_sync(0xffffffffu, mine, i), l = __shfl_sync(0xffffffffu, ml.y, i);
-      // a part that saw nothing has left no output
-      if (w > 0.f) {
-        sum += w * l;
-        const float *o = p.part + place(base + i) * D + lane * kVec;
-#pragma unroll
-        for (int e = 0; e < kVec; e += 2) {
-          const float2 x = *reinterpret_cast<const float2 *>(o + e);
-          acc[e] += w * x.x;
-          acc[e + 1] += w * x.y;
-        }
-      }
+      for (int e = 0; e < 16; ++e) s_acc[warp][e][lane] = j.acc[e];
+      s_acc[warp][16][lane] = j.top;
+      s_acc[warp][17][lane] = j.sum;
     }
-  }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  const int tok = q.q0 + t0 + row / p.s.group, head = cut.y * p.s.group + row % p.s.group;
-  T *out = static_cast<T *>(p.out) + tok * p.out_stride[0] + head * p.out_stride[1] + lane * kVec;
+    __syncthreads();
+    if (warp > 0 || row >= rows) return;
+    const int n = min(parts, 8);
+    for (int w = 1; w < n; ++w) j.top = fmaxf(j.top, s_acc[w][16][lane]);
+    const float ref = j.top == -INFINITY ? 0.f : j.top;
+    j.sum = 0.f;
 #pragma unroll
-  for (int e = 0; e < kVec; ++e)
-    if (lane * kVec + e < p.head_dim) out[e] = static_cast<T>(acc[e] * inv);  // rounded once, to nearest
-  if (p.m_out && lane == 0) p.m_out[static_cast<long long>(tok) * p.heads + head] = sum > 0.f ? top + log2f(sum) : -INFINITY;
+    for (int e = 0; e < 16; ++e) j.acc[e] = 0.f;
+    for (int w = 0; w < n; ++w) {
+      const float f = fast_exp2(s_acc[w][16][lane] - ref);
+      j.sum += f * s_acc[w][17][lane];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) j.acc[e] += f * s_acc[w][e][lane];
+    }
+  } else {
+    if (row >= rows) return;
+    j = join_parts<D>(p, c, 0, 1, parts, row, col);
+  }
+  const float inv = j.sum > 0.f ? 1.f / j.sum : 0.f;
+  const int tok = q.q0 + t0 + row / p.s.group, head = cut.y * p.s.group + row % p.s.group;
+  struct alignas(16) Eight { T x[8]; } y[2];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) y[e / 8].x[e % 8] = static_cast<T>(j.acc[e] * inv);  // rounded once, to nearest
+  Eight *out = reinterpret_cast<Eight *>(static_cast<T *>(p.out) + tok * p.out_stride[0] + head * p.out_stride[1] + col);
+  out[0] = y[0];
+  out[1] = y[1];
+  if (p.m_out && col == 0)
+    p.m_out[static_cast<long long>(tok) * p.heads + head] = j.sum > 0.f ? j.top + log2f(j.sum) : -INFINITY;
 }
 
 }  // namespace txp

@@ -4,10 +4,14 @@
 // an S and an O accumulator in tensor memory each, a TMA producer warp, a tcgen05.mma warp that serves the sub-tiles in
 // turn), made persistent and fed from pages:
 //   * a sub-tile's 128 rows are T new tokens x the G query heads of one key head (T = 128 / G, rows left over are zero), so
-//     that a group reads its keys and values once; one TMA box {64, G, T} brings them
+//     that a group reads its keys and values once; one TMA box {64, G, T} brings them. The two sub-tiles take every second
+//     token each, so that under a causal mask both see the same blocks: with the earlier tokens in one and the later ones
+//     in the other, the one was done a block before the other in every tile and waited for it from then on (12 prompts of
+//     1024 tokens, 12 heads of 64: 84 us, this 76 us)
 //   * K and V tiles of 128 tokens arrive as one TMA copy per page and 64 columns, page coordinates from the page table
-//   * a CTA walks its stretch of the work line (paged_schedule.cuh), so the barriers' phases run on from tile to tile; a
-//     tile of which it has only some blocks leaves fp32 partial results to the joining kernel
+//   * a CTA walks its share of the work (paged_schedule.cuh), so the barriers' phases run on from tile to tile; a scheduler
+//     warp works the next tiles out ahead of the others (each role doing that by itself took over 1 us a tile); a tile of
+//     which the CTA has only some blocks leaves fp32 partial results to the joining kernel
 //   * rows of V that no row of the tile sees may hold anything: the MMA warp zeroes them in shared memory before the
 //     product (0 * NaN must not reach O); scores of keys that a row does not see are replaced, not added to
 // Every wait on an mbarrier is bounded in time, as there.
@@ -18,10 +22,25 @@
 
 namespace txp {
 
-constexpr int kTileThreads = txa::kAttnThreads;
+constexpr int kSchedulerWarp = 10;
+constexpr int kTileThreads = 352;
+constexpr int kItems = 4;  // tiles that the scheduler warp may be ahead
+
+// One tile of a CTA's work, as its roles take it.
+struct TileItem {
+  int tok0, tokens;    // new tokens [tok0, tok0 + tokens) of the batch
+  int pos0;            // position of the first in its sequence
+  int head, seq;
+  int lo, hi, kv;      // keys that some row sees: [lo, hi); the sequence's keys
+  int block, blocks;   // KV blocks [block, block + blocks) of the sequence
+  int whole;           // not a part of a cut tile
+  int slot;            // of the partial result
+  int more;            // 0: the work is done
+  int pad[3];
+};
 
 struct TileParams {
-  CUtensorMap tmap_q;          // {head_dim, heads, tokens}, box {64, G, T}
+  CUtensorMap tmap_q, tmap_q2; // {head_dim, heads, tokens}, box {64, G, T} of consecutive tokens and of every second one
   CUtensorMap tmap_k, tmap_v;  // {64 columns, slots, column groups, heads, pages}, box {64, rows, 1, 1, 1}
   Sched s;
   void *out;
@@ -30,7 +49,7 @@ struct TileParams {
   const int32_t *table;
   long long table_stride;
   int4 *borders;
-  float *part;
+  float4 *part;
   float2 *ml;
   unsigned long long wait_limit_ns;
   float qk_scale;
@@ -53,19 +72,12 @@ struct TileCtl {
   uint64_t q_full, q_empty;
   uint64_t kv_full[6], kv_empty[6];
   uint64_t s_full[2], s_free[2], p_full[2], o_done[2];
+  uint64_t item_full[kItems], item_empty[kItems];
   uint64_t drain;
+  TileItem item[kItems];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
-
-// Blocks [0, n) of a walk's part that sub-tile t takes: its rows see fewer keys than the tile's last ones.
-__device__ __forceinline__ int sub_blocks(const Sched &s, const Walk &w, int t, int sub_tokens) {
-  const int a = w.t.t0 + t * sub_tokens, b = min(a + sub_tokens, w.t.t1);
-  if (a >= w.t.t1) return 0;
-  const int hi = s.causal ? max(w.t.off + b, 0) : w.q.kv;
-  const int end = min(((hi + 127) >> 7) - w.t.blk0, w.to);
-  return max(end - w.from, 0);
-}
 
 template <bool kBf16, int D>
 __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ TileParams p) {
@@ -95,10 +107,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       mbar_init(smem_u32(&ctl.p_full[t]), 128);
       mbar_init(smem_u32(&ctl.o_done[t]), 1);
     }
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(smem_u32(&ctl.item_full[i]), 1);
+      mbar_init(smem_u32(&ctl.item_empty[i]), 10);  // every warp but the scheduler
+    }
     mbar_init(smem_u32(&ctl.drain), 1);
     ctl.abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&p.tmap_q);
+    tma_prefetch_desc(&p.tmap_q2);
     tma_prefetch_desc(&p.tmap_k);
     tma_prefetch_desc(&p.tmap_v);
   }
@@ -117,7 +134,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   }
   grid_dep_wait();
   tc_fence_before();
-  const bool work = find_stretch<kTileThreads>(p.s, &sched, p.borders);  // syncs the CTA
+  find_work<kTileThreads, true>(p.s, &sched, p.borders, reinterpret_cast<int *>(tile_smem_raw + (p_addr0 - smem_u32(tile_smem_raw))));
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = ctl.tmem_base;
 
@@ -125,10 +143,50 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   ac.flag = &ctl.abort_flag;
   ac.status = p.s.status;
   ac.limit_ns = p.wait_limit_ns;
-  Walk w;
 
-  if (!work) {
-    // nothing to do but to give the tensor memory back
+  // The next tile, read into registers; false when there is none (or the wait for it ran out).
+  TileItem w;
+  uint32_t item_count = 0;
+  auto next_item = [&]() -> bool {
+    const uint32_t i = item_count % kItems;
+    if (!warp_mbar_poll(smem_u32(&ctl.item_full[i]), (item_count / kItems) & 1u, ac, kTimeout, lane)) return false;
+    w = ctl.item[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[i]));
+    ++item_count;
+    return w.more != 0;
+  };
+
+  if (warp == kSchedulerWarp) {
+    // ------------------------------ scheduler: walks the CTA's work ahead of the others ------------------------------
+    Walk walk;
+    uint32_t count = 0;
+    for (bool more = walk.start(p.s, &sched), last = false; !last; more = more && walk.next(p.s, &sched), ++count) {
+      last = !more;
+      const uint32_t i = count % kItems;
+      if (!warp_mbar_poll(smem_u32(&ctl.item_empty[i]), ((count / kItems) & 1u) ^ 1u, ac, kTimeout, lane)) break;
+      if (lane == 0) {
+        TileItem x = {};
+        if (more) {
+          x.tok0 = walk.q.q0 + walk.t.t0;
+          x.tokens = walk.t.t1 - walk.t.t0;
+          x.pos0 = walk.t.off + walk.t.t0;
+          x.head = walk.at.h;
+          x.seq = walk.at.b;
+          x.lo = walk.t.lo;
+          x.hi = walk.t.hi;
+          x.kv = walk.q.kv;
+          x.block = walk.t.blk0 + walk.from;
+          x.blocks = walk.to - walk.from;
+          x.whole = walk.whole();
+          x.slot = static_cast<int>(walk.slot());
+          x.more = 1;
+        }
+        ctl.item[i] = x;
+        mbar_arrive(smem_u32(&ctl.item_full[i]));
+      }
+      __syncwarp();
+    }
   } else if (warp == txa::kProducerWarp) {
     // ------------------------------ TMA producer ------------------------------
     const bool issuer = elect_one();
@@ -136,8 +194,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     bool ok = true;
     const int boxes = 128 >> p.box_shift;  // copies of one atom of a tile
     const uint32_t box_bytes = 128u << p.box_shift;
-    for (bool more = w.start(p.s, &sched); more && ok; more = w.next(p.s)) {
-      const int nb = w.to - w.from;
+    while (ok && next_item()) {
+      const int nb = w.blocks;
       if (nb <= 0) continue;
       if (!warp_mbar_poll(smem_u32(&ctl.q_empty), (items & 1u) ^ 1u, ac, kTimeout, lane)) {
         ok = false;
@@ -145,44 +203,63 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       }
       if (issuer) {
         const uint32_t bar = smem_u32(&ctl.q_full);
-        const int active = w.t.t1 - w.t.t0 > p.sub_tokens ? 2 : 1;
+        const int active = w.tokens > p.sub_tokens ? 2 : 1;
         mbar_arrive_expect_tx(bar, active * kAtoms * p.sub_tokens * p.s.group * 128);
         for (int t = 0; t < active; ++t)
           for (int a = 0; a < kAtoms; ++a)
-            tma_load_3d(q_addr0 + t * tile_bytes + a * kAtomBytes, &p.tmap_q, a * 64, w.at.h * p.s.group,
-                        w.q.q0 + w.t.t0 + t * p.sub_tokens, bar);
+            tma_load_3d(q_addr0 + t * tile_bytes + a * kAtomBytes, active == 2 ? &p.tmap_q2 : &p.tmap_q, a * 64,
+                        w.head * p.s.group, w.tok0 + t, bar);
       }
       __syncwarp();
       ++items;
-      const int32_t *row = p.table + w.at.b * p.table_stride;
-      const int first_page = w.t.lo >> p.page_shift, last_page = (w.t.hi - 1) >> p.page_shift;
-      int window[2] = {-1, -1}, page_reg[2] = {0, 0};  // for K and V: 32 entries of the page table, one a lane
-      // lane: box and atom of the tile
-      const int box = lane & (boxes - 1), atom = lane >> (7 - p.box_shift);
-      auto load_tile = [&](int j, int is_v) {
-        const int tok0 = (w.t.blk0 + w.from + j) * 128;
-        const int tok = tok0 + (box << p.box_shift), page = tok >> p.page_shift;
-        const int want_window = (tok0 >> p.page_shift) >> 5;
-        if (window[is_v] != want_window) {
-          window[is_v] = want_window;
-          const int at = want_window * 32 + lane;
-          page_reg[is_v] = at >= first_page && at <= last_page ? row[at] : 0;
-          if (page_reg[is_v] < 0 || page_reg[is_v] >= p.num_pages) atomicOr(p.s.status, kBadPage);
+      const int32_t *row = p.table + w.seq * p.table_stride;
+      const int first_page = w.lo >> p.page_shift, last_page = (w.hi - 1) >> p.page_shift;
+      // The page table, 32 entries (one a lane) at a time: the window that K is in, the one before it (V follows one block
+      // behind) and the one after it, whose load is under way long before it is needed.
+      auto entries = [&](int win) {
+        const int at = win * 32 + lane;
+        return at >= first_page && at <= last_page ? row[at] : 0;
+      };
+      int window = (w.block * 128 >> p.page_shift) >> 5;
+      int before = 0, cur = entries(window), after = entries(window + 1);
+      auto check = [&] {
+        if (cur < 0 || cur >= p.num_pages) atomicOr(p.s.status, kBadPage);
+      };
+      check();
+      // All lanes walk the copies of a tile together, one issues (with one copy a lane, the warp went through them one by one
+      // with everything of a copy set up anew: no faster, and 16 copies at 16-token pages)
+      auto load_tile = [&](int j, bool is_v) {
+        const int tok0 = (w.block + j) * 128;
+        const int want = (tok0 >> p.page_shift) >> 5;
+        if (want > window) {  // by K only, one at a time
+          window = want;
+          before = cur;
+          cur = after;
+          after = entries(window + 1);
+          check();
         }
-        const int id = __shfl_sync(0xffffffffu, page_reg[is_v], page & 31);
-        const bool wanted = atom < kAtoms && tok < w.t.hi && tok + (1 << p.box_shift) > w.t.lo;
-        const uint32_t count = __popc(__ballot_sync(0xffffffffu, wanted));
+        const int ids = want == window ? cur : before;
+        const int b0 = max(w.lo - tok0, 0) >> p.box_shift;  // copies [b0, b1) hold keys that are seen
+        const int b1 = min((w.hi - tok0 + (1 << p.box_shift) - 1) >> p.box_shift, boxes);
         const uint32_t slot = issued % kStages;
+        const uint32_t bar = smem_u32(&ctl.kv_full[slot]);
+        const CUtensorMap *map = is_v ? &p.tmap_v : &p.tmap_k;
+        const uint32_t dst = kv_addr0 + slot * tile_bytes;
         if (!warp_mbar_poll(smem_u32(&ctl.kv_empty[slot]), ((issued / kStages) & 1u) ^ 1u, ac, kTimeout, lane)) {
           ok = false;
           return;
         }
-        const uint32_t bar = smem_u32(&ctl.kv_full[slot]);
-        if (lane == 0) mbar_arrive_expect_tx(bar, count * box_bytes);
-        __syncwarp();
-        if (wanted)
-          tma_load_5d(kv_addr0 + slot * tile_bytes + atom * kAtomBytes + box * box_bytes, is_v ? &p.tmap_v : &p.tmap_k, 0,
-                      tok & ((1 << p.page_shift) - 1), atom, w.at.h, id, bar);
+        if (issuer) mbar_arrive_expect_tx(bar, (b1 - b0) * kAtoms * box_bytes);
+        for (int b = b0; b < b1; ++b) {
+          const int tok = tok0 + (b << p.box_shift);
+          const int id = __shfl_sync(0xffffffffu, ids, (tok >> p.page_shift) & 31);
+          const int in_page = tok & ((1 << p.page_shift) - 1);
+          if (issuer) {
+#pragma unroll
+            for (int a = 0; a < kAtoms; ++a)
+              tma_load_5d(dst + a * kAtomBytes + b * box_bytes, map, 0, in_page, a, w.head, id, bar);
+          }
+        }
         __syncwarp();
         ++issued;
       };
@@ -190,10 +267,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         ok = false;
         break;
       }
-      load_tile(0, 0);
+      load_tile(0, false);
       for (int j = 0; ok && j < nb; ++j) {
-        if (j + 1 < nb) load_tile(j + 1, 0);
-        if (ok) load_tile(j, 1);
+        if (j + 1 < nb) load_tile(j + 1, false);
+        if (ok) load_tile(j, true);
       }
     }
     if (!ok || ctl.abort_flag) {  // copies in flight land before the shared memory goes away
@@ -227,8 +304,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     // A V tile: its rows that nobody sees are zeroed before they are multiplied.
     auto take_v = [&](int j) -> uint32_t {
       const uint32_t slot = take();
-      const int tok0 = (w.t.blk0 + w.from + j) * 128;
-      const int a = max(w.t.lo - tok0, 0), b = min(w.t.hi - tok0, 128);
+      const int tok0 = (w.block + j) * 128;
+      const int a = max(w.lo - tok0, 0), b = min(w.hi - tok0, 128);
       if (ok && (a > 0 || b < 128)) {
         for (int at = 0; at < kAtoms; ++at) {
           const uint32_t base = kv_addr0 + slot * tile_bytes + at * kAtomBytes;
@@ -279,10 +356,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       ++p_count[t];
     };
 
-    for (bool more = w.start(p.s, &sched); more && ok; more = w.next(p.s)) {
-      const int nb = w.to - w.from;
+    while (ok && next_item()) {
+      const int nb = w.blocks;
       if (nb <= 0) continue;
-      const int n_blk[2] = {sub_blocks(p.s, w, 0, p.sub_tokens), sub_blocks(p.s, w, 1, p.sub_tokens)};
+      const int n_blk[2] = {nb, w.tokens > p.sub_tokens ? nb : 0};
       // S of block j: after the accumulator's last S has been read into registers (one tile's last before the next one's first)
       auto next_s = [&](int t, int j, uint32_t k_slot) {
         if (j >= n_blk[t]) return;
@@ -378,18 +455,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     const int tok_in_sub = r / p.s.group, g = r - tok_in_sub * p.s.group;
     uint32_t count = 0;  // blocks of this sub-tile so far
     bool ok = true;
-    for (bool more = w.start(p.s, &sched); more && ok; more = w.next(p.s)) {
-      const int n = sub_blocks(p.s, w, t, p.sub_tokens);
-      const int first = w.t.t0 + t * p.sub_tokens;  // the sub-tile's tokens: [first, last)
-      const int last = min(first + p.sub_tokens, w.t.t1);
-      const int tok = first + tok_in_sub;
-      const bool valid = r < sub_rows && tok < last;
-      const int pos = w.t.off + tok;
-      const int hi_r = !valid ? 0 : p.s.causal ? pos + 1 : w.q.kv;
+    while (ok && next_item()) {
+      const bool both = w.tokens > p.sub_tokens;  // a tile of few tokens is sub-tile 0's alone
+      const int n = t == 0 || both ? w.blocks : 0;
+      const int rel = both ? t + 2 * tok_in_sub : tok_in_sub;  // this row's token of the tile's
+      const bool valid = r < sub_rows && rel < w.tokens && (t == 0 || both);
+      const int pos = w.pos0 + rel;
+      const int hi_r = !valid ? 0 : p.s.causal ? pos + 1 : w.kv;
       const int lo_r = p.s.window ? pos + 1 - p.s.window : 0;
       // blocks inside [inner_lo, inner_hi) are seen whole by every row: the loop's unmasked part
-      const int inner_hi = p.s.causal ? w.t.off + first + 1 : w.q.kv;
-      const int inner_lo = p.s.window ? w.t.off + last - p.s.window : 0;
+      const int inner_hi = p.s.causal ? w.pos0 + t + 1 : w.kv;
+      const int inner_lo = p.s.window ? w.pos0 + w.tokens - p.s.window : 0;
       float m_i = -INFINITY, l_i = 0.f;
       for (int j = 0; j < n; ++j, ++count) {
         if (!warp_mbar_poll(smem_u32(&ctl.s_full[t]), count & 1u, ac, kTimeout, lane)) {
@@ -405,10 +481,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         tmem_ld_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(&ctl.s_free[t]));
-        const int col0 = (w.t.blk0 + w.from + j) * 128;
+        const int col0 = (w.block + j) * 128;
         if (col0 + 128 > inner_hi || col0 < inner_lo) {
+          // by one word of bits for 32 columns: a third of the instructions of two compares for each score, and what this
+          // code takes is mostly its own fetching (12 prompts, of 150 to 1500 tokens: 112 us with compares, 102)
+          const int hi = hi_r - col0, lo = lo_r - col0;
 #pragma unroll
-          for (int i = 0; i < 128; ++i) s[i] = col0 + i < hi_r && col0 + i >= lo_r ? s[i] : 0xff800000u;  // -inf
+          for (int c = 0; c < 4; ++c) {
+            const int h = min(max(hi - c * 32, 0), 32), l = min(max(lo - c * 32, 0), 32);
+            const uint32_t seen = (h == 32 ? 0xffffffffu : (1u << h) - 1u) & (l == 32 ? 0u : 0xffffffffu << l);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[c * 32 + i] = (seen & (1u << i)) ? s[c * 32 + i] : 0xff800000u;  // -inf
+          }
         }
         const float mx = txa::row_block_max<false>(s, 0, 0);
         // the reference moves only when the block's maximum passes it by 2^8 (see the forward kernel)
@@ -450,13 +534,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         if (!ok) break;
         tc_fence_after();
       }
-      if (first >= w.t.t1) continue;
+      if (t == 1 && !both) continue;
       const float inv_l = l_i > 0.f ? 1.0f / l_i : 0.f;
-      const bool whole = w.whole();
-      const int head = w.at.h * p.s.group + g;
-      const long long part_row = (static_cast<long long>(blockIdx.x) * 2 + w.slot()) * p.part_rows + t * sub_rows + r;
+      const bool whole = w.whole != 0;
+      const int head = w.head * p.s.group + g, tok = w.tok0 + rel;
+      const int part_row = rel * p.s.group + g;
       using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
-      T *o_row = static_cast<T *>(p.out) + (w.q.q0 + tok) * p.out_stride[0] + head * p.out_stride[1];
+      const long long o_row = tok * p.out_stride[0] + head * p.out_stride[1];
+      const uint32_t stage = p_row - static_cast<uint32_t>((r & 7) * 128 + (r >> 3) * 1024);  // this sub-tile's P
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -467,26 +552,42 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        if (valid && whole) {
+        if (whole) {
+          // rows go out through P's place in shared memory, so that a store instruction covers whole rows
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               x[i] = txa::pack_pair<kElt>(__uint_as_float(o[q * 8 + 2 * i]) * inv_l, __uint_as_float(o[q * 8 + 2 * i + 1]) * inv_l);
-            if (c * 32 + q * 8 < p.head_dim) *reinterpret_cast<uint4 *>(o_row + c * 32 + q * 8) = make_uint4(x[0], x[1], x[2], x[3]);
+            st_shared_v4(stage + (c >> 1) * kAtomBytes + txa::swz_off(r, (c & 1) * 4 + q), x[0], x[1], x[2], x[3]);
           }
         } else if (valid) {
-          float *dst = p.part + part_row * D + c * 32;
+          float4 *dst = p.part + (static_cast<long long>(w.slot) * (D / 4) + c * 8) * p.part_rows + part_row;
 #pragma unroll
           for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<uint4 *>(dst + q * 4) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+            dst[static_cast<long long>(q) * p.part_rows] =
+                make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3]));
+        }
+        __syncwarp();
+      }
+      if (whole) {
+        constexpr int kLanes = D / 8;  // lanes of a row, 16 bytes each
+        const uint32_t valid_rows = __ballot_sync(0xffffffffu, valid);
+#pragma unroll 4
+        for (int i = 0; i < kLanes; ++i) {
+          const int rr = i * (32 / kLanes) + lane / kLanes, c16 = lane % kLanes;
+          const long long at = __shfl_sync(0xffffffffu, o_row, rr);
+          uint4 x;
+          const uint32_t from = stage + (c16 >> 3) * kAtomBytes + txa::swz_off(quarter * 32 + rr, c16 & 7);
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(from) : "memory");
+          if ((valid_rows >> rr & 1u) && c16 * 8 < p.head_dim) *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + at + c16 * 8) = x;
         }
         __syncwarp();
       }
       if (valid) {
-        if (!whole) p.ml[part_row] = make_float2(m_i, l_i);
-        else if (p.m_out) p.m_out[static_cast<long long>(w.q.q0 + tok) * p.heads + head] = l_i > 0.f ? m_i + log2f(l_i) : -INFINITY;
+        if (!whole) p.ml[static_cast<long long>(w.slot) * p.part_rows + part_row] = make_float2(m_i, l_i);
+        else if (p.m_out) p.m_out[static_cast<long long>(tok) * p.heads + head] = l_i > 0.f ? m_i + log2f(l_i) : -INFINITY;
       }
     }
   }
