@@ -72,7 +72,7 @@ RowShape row_shape(int kernel_d, int group, int max_q) {
   const long long rows = static_cast<long long>(group) * (max_q > 0 ? max_q : 1);
   if (rows <= 16) return {1, 4, kernel_d == 256 ? 1 : 2};
   if (rows <= 32) return {2, 4, 1};
-  return {4, 2, 1};
+  return {4, 2, 1};  // head dimension 256 only
 }
 
 int sm_count() {
@@ -118,8 +118,9 @@ int make_plan(const tx_paged_view *cache, const tx_paged_attn_problem *pr, Plan 
   if (max_q > pr->tokens) max_q = pr->tokens;
   plan->shape = row_shape(plan->kernel_d, plan->group, max_q);
   // 128-row tiles on tcgen05 for head dimensions up to 128 (256 columns of O for two sub-tiles do not fit tensor memory
-  // next to S); up to 64 rows the streaming kernel
-  plan->tiled = plan->kernel_d <= 128 && static_cast<long long>(plan->group) * max_q > 64;
+  // next to S); up to 32 rows the streaming kernel. Measured, 16 sequences of up to 4100 tokens, 32 + 8 heads of 128, tiles
+  // against streams: 32 rows 71 us and 57, 64 rows 66 us and 84.
+  plan->tiled = plan->kernel_d <= 128 && static_cast<long long>(plan->group) * max_q > 32;
   plan->rows = plan->tiled ? 256 : plan->shape.mt * 16;
   plan->ctas = sm_count() * (plan->tiled ? 1 : plan->shape.per_sm);
   plan->borders_bytes = (static_cast<size_t>(plan->ctas) * 16 + 255) / 256 * 256;
@@ -174,13 +175,11 @@ int launch_row_any(const Plan &plan, const RowParams &prm, cudaStream_t s) {
   // ring: 96 KB a CTA where two share an SM, up to 192 KB where one has it
   if (plan.kernel_d == 64) {
     if (mt == 1) return launch_row<kBf16, 64, 1, 4, 6, 2>(prm, plan.ctas, s);
-    if (mt == 2) return launch_row<kBf16, 64, 2, 4, 8, 1>(prm, plan.ctas, s);
-    return launch_row<kBf16, 64, 4, 2, 8, 1>(prm, plan.ctas, s);
+    return launch_row<kBf16, 64, 2, 4, 8, 1>(prm, plan.ctas, s);
   }
   if (plan.kernel_d == 128) {
     if (mt == 1) return launch_row<kBf16, 128, 1, 4, 3, 2>(prm, plan.ctas, s);
-    if (mt == 2) return launch_row<kBf16, 128, 2, 4, 6, 1>(prm, plan.ctas, s);
-    return launch_row<kBf16, 128, 4, 2, 6, 1>(prm, plan.ctas, s);
+    return launch_row<kBf16, 128, 2, 4, 6, 1>(prm, plan.ctas, s);
   }
   if (mt == 1) return launch_row<kBf16, 256, 1, 4, 3, 1>(prm, plan.ctas, s);
   if (mt == 2) return launch_row<kBf16, 256, 2, 4, 3, 1>(prm, plan.ctas, s);
@@ -283,7 +282,7 @@ int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_problem *
   sched.block_shift = 6;
   sched.tile_cost = 2;
   sched.min_part = 2;
-  sched.min_share = 4;
+  sched.min_share = 3;
   sched.waves = kMaxWaves;
   sched.status = status;
 

@@ -259,51 +259,67 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
             mma_16816<kBf16>(s[2 * i], qf[kk], b[0], b[1]);
             mma_16816<kBf16>(s[2 * i + 1], qf[kk], b[2], b[3]);
           }
-        // ---- softmax: scores in log2 units against the running maximum ----
+        if (edge) {
+          // V at keys that no row of the tile sees may be anything, NaN included: 0 * NaN must not reach O. (Warps of other
+          // rows write the same zeros.)
+#pragma unroll
+          for (int i = 0; i < kSlabs; ++i) {
+            const int key = blk_tok + ks * kTok + i * 16;
+            if (key >= w.t.lo && key + 16 <= w.t.hi) continue;
+            for (int x = lane; x < 16 * 8 * kGroups; x += 32) {
+              const int tok = (x >> 3) & 15;
+              if (key + tok < w.t.lo || key + tok >= w.t.hi)
+                st_shared_v4(v_base + slab[i] + (x >> 7) * group_bytes + tok * 128u + (x & 7) * 16u, 0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async();  // TMA writes the slot next
+          __syncwarp();
+          // scores of keys that the row does not see
+#pragma unroll
+          for (int i = 0; i < kSlabs * 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = blk_tok + ks * kTok + i * 8 + l4 * 2 + (e & 1);
+              s[i][e] = key < hi_r[e >> 1] && key >= lo_r[e >> 1] ? s[i][e] : -INFINITY;
+            }
+        }
+        // ---- softmax, in log2 units, against the running maximum ----
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < kSlabs * 2; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = s[i][e] * p.qk_scale;
-            if (edge) {
-              const int key = blk_tok + ks * kTok + i * 8 + l4 * 2 + (e & 1);
-              x = key < hi_r[e >> 1] && key >= lo_r[e >> 1] ? x : -INFINITY;
-            }
-            s[i][e] = x;
-            mx[e >> 1] = fmaxf(mx[e >> 1], x);
-          }
+          for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[i][e]);
         float ref[2];
         bool grow = false;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)) * p.qk_scale;
           // the reference moves only when a score passes it by 2^8 (values stay below 2^8 times the exact ones: nothing is
           // lost in fp32, and P rounds relative to itself)
-          const bool up = mx[e] > m[e] + 8.f || m[e] == -INFINITY;
-          const float next = up ? fmaxf(m[e], mx[e]) : m[e];
-          grow |= next != m[e];
-          ref[e] = next == -INFINITY ? 0.f : next;
-          const float a = next != m[e] ? fast_exp2(m[e] - ref[e]) : 1.f;
-          l[e] *= a;
-          m[e] = next;
-          mx[e] = a;  // from here on: the factor of what was summed before
+          grow |= mx[e] > m[e] + 8.f;
         }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            o[i][0] *= mx[0];
-            o[i][1] *= mx[0];
-            o[i][2] *= mx[1];
-            o[i][3] *= mx[1];
+          for (int e = 0; e < 2; ++e) {
+            const float next = mx[e] > m[e] + 8.f ? mx[e] : m[e];
+            const float a = next != m[e] ? fast_exp2(m[e] - next) : 1.f;
+            m[e] = next;
+            l[e] *= a;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+              o[i][2 * e] *= a;
+              o[i][2 * e + 1] *= a;
+            }
           }
         }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) ref[e] = m[e] == -INFINITY ? 0.f : -m[e];
         uint32_t pf[kSlabs][4];
 #pragma unroll
         for (int i = 0; i < kSlabs * 2; ++i) {
-          const float e0 = fast_exp2(s[i][0] - ref[0]), e1 = fast_exp2(s[i][1] - ref[0]);
-          const float e2 = fast_exp2(s[i][2] - ref[1]), e3 = fast_exp2(s[i][3] - ref[1]);
+          const float e0 = fast_exp2(fmaf(s[i][0], p.qk_scale, ref[0])), e1 = fast_exp2(fmaf(s[i][1], p.qk_scale, ref[0]));
+          const float e2 = fast_exp2(fmaf(s[i][2], p.qk_scale, ref[1])), e3 = fast_exp2(fmaf(s[i][3], p.qk_scale, ref[1]));
           l[0] += e0 + e1;
           l[1] += e2 + e3;
           pf[i >> 1][(i & 1) * 2] = pack2<kBf16>(e0, e1);
@@ -311,31 +327,14 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
         }
         // ---- O += P V ----
 #pragma unroll
-        for (int i = 0; i < kSlabs; ++i) {
-          uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-          if (edge) {
-            // V at keys that no row of the tile sees may be anything, NaN included: 0 * NaN must not reach O
-            const int key = blk_tok + ks * kTok + i * 16 + l4 * 2;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int a = key + e * 8;
-              keep[e] = (a >= w.t.lo && a < w.t.hi ? 0xffffu : 0u) | (a + 1 >= w.t.lo && a + 1 < w.t.hi ? 0xffff0000u : 0u);
-            }
-          }
+        for (int i = 0; i < kSlabs; ++i)
 #pragma unroll
           for (int dd = 0; dd < D / 16; ++dd) {
             uint32_t b[4];
             ldmatrix_x4_trans(v_base + slab[i] + (dd >> 2) * group_bytes + v_row + ((((dd & 3) * 2 + v_chunk) ^ x7) << 4), b);
-            if (edge) {
-              b[0] &= keep[0];
-              b[1] &= keep[1];
-              b[2] &= keep[0];
-              b[3] &= keep[1];
-            }
             mma_16816<kBf16>(o[2 * dd], pf[i], b[0], b[1]);
             mma_16816<kBf16>(o[2 * dd + 1], pf[i], b[2], b[3]);
           }
-        }
         give(slot);
       }
 
