@@ -325,8 +325,7 @@ int tx_pages_free(const tx_pages_state *st, const int32_t *rows, int32_t n, void
   if (n == 0) return TXD_OK;
   PagesParams p = {};
   if ((rc = pages_params(st, nullptr, &p))) return rc;
-  pages_free_kernel<<<static_cast<unsigned>(n), 256, 0, static_cast<cudaStream_t>(stream)>>>(p, rows);
-  TXP_CUDA(cudaGetLastError());
+  TXP_CUDA(launch(pages_free_kernel, dim3(n), dim3(256), 0, static_cast<cudaStream_t>(stream), p, rows));
   count_launches(1);
   return TXD_OK;
 }
@@ -340,10 +339,8 @@ int tx_pages_fork(const tx_pages_state *st, const int32_t *dst, const int32_t *s
   PagesParams p = {};
   if ((rc = pages_params(st, workspace, &p))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  pages_fork_take_kernel<<<static_cast<unsigned>(n), 256, 0, s>>>(p, dst, src, n);
-  TXP_CUDA(cudaGetLastError());
-  pages_fork_put_kernel<<<static_cast<unsigned>(n), 256, 0, s>>>(p, dst);
-  TXP_CUDA(cudaGetLastError());
+  TXP_CUDA(launch(pages_fork_take_kernel, dim3(n), dim3(256), 0, s, p, dst, src, n));
+  TXP_CUDA(launch(pages_fork_put_kernel, dim3(n), dim3(256), 0, s, p, dst));
   count_launches(2);
   return TXD_OK;
 }
@@ -361,11 +358,9 @@ int tx_pages_reserve(const tx_pages_state *st, const int32_t *rows, const int32_
   if ((rc = pages_params(st, workspace, &p))) return rc;
   if ((rc = set_plan_smem())) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const size_t smem = (2 * static_cast<size_t>(n) + (st->rows + 31) / 32) * 4;
-  pages_reserve_plan_kernel<<<1, kPlanThreads, smem, s>>>(p, rows, counts, n);
-  TXP_CUDA(cudaGetLastError());
-  pages_copy_kernel<<<copy_grid(st, n), 256, 0, s>>>(p);
-  TXP_CUDA(cudaGetLastError());
+  const size_t smem = (4 * static_cast<size_t>(n) + (st->rows + 31) / 32) * 4;
+  TXP_CUDA(launch(pages_reserve_plan_kernel, dim3(1), dim3(kPlanThreads), smem, s, p, rows, counts, n));
+  TXP_CUDA(launch(pages_copy_kernel, dim3(copy_grid(st, n)), dim3(256), 0, s, p));
   count_launches(2);
   return TXD_OK;
 }
@@ -377,10 +372,8 @@ int tx_pages_compact(const tx_pages_state *st, void *workspace, void *stream) {
   PagesParams p = {};
   if ((rc = pages_params(st, workspace, &p))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  pages_compact_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
-  TXP_CUDA(cudaGetLastError());
-  pages_compact_move_kernel<<<copy_grid(st, st->num_pages), 256, 0, s>>>(p);
-  TXP_CUDA(cudaGetLastError());
+  TXP_CUDA(launch(pages_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p));
+  TXP_CUDA(launch(pages_compact_move_kernel, dim3(copy_grid(st, st->num_pages)), dim3(256), 0, s, p));
   count_launches(2);
   return TXD_OK;
 }
@@ -413,8 +406,7 @@ int tx_pages_copy(const tx_pages_state *st, const int32_t *src, const int32_t *d
       pp.pair[2 * i] = src[at + i];
       pp.pair[2 * i + 1] = dst[at + i];
     }
-    pages_copy_listed_kernel<<<copy_grid(st, count), 256, 0, static_cast<cudaStream_t>(stream)>>>(p, pp, count);
-    TXP_CUDA(cudaGetLastError());
+    TXP_CUDA(launch(pages_copy_listed_kernel, dim3(copy_grid(st, count)), dim3(256), 0, static_cast<cudaStream_t>(stream), p, pp, count));
     count_launches(1);
   }
   return TXD_OK;

@@ -130,23 +130,6 @@ int make_plan(const tx_paged_view *cache, const tx_paged_attn_problem *pr, Plan 
   return TXD_OK;
 }
 
-// The programmatic attribute lets a kernel be scheduled while its predecessor drains; it waits for it before it touches
-// memory (griddepcontrol.wait).
-template <typename P>
-cudaError_t launch(void (*kernel)(P), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const P &p) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 // The kernel's shared-memory limit is raised once per device.
 template <typename P>
 cudaError_t allow_smem(void (*kernel)(P), int bytes, std::atomic<uint64_t> *done) {
@@ -208,9 +191,10 @@ uint32_t mma_idesc(bool bf16, bool b_mn_major, int n) {
 
 template <typename T, int D>
 int launch_join_d(const Plan &plan, const JoinParams &j, cudaStream_t s) {
-  const int units = (plan.rows + 31) / 32 * (D / 16);  // warps of a tile, or blocks where few rows are joined
-  if (plan.rows <= 64) TXP_CUDA(launch(paged_join_kernel<T, D, true>, dim3(j.ctas - 1, units), dim3(256), 0, s, j));
-  else TXP_CUDA(launch(paged_join_kernel<T, D, false>, dim3(j.ctas - 1, (units + 7) / 8), dim3(256), 0, s, j));
+  const unsigned borders = static_cast<unsigned>(j.ctas - 1), row_groups = static_cast<unsigned>(plan.rows + 31) / 32;
+  if (plan.rows == 16) TXP_CUDA(launch(paged_join_kernel<T, D, 16>, dim3(borders), dim3(D * 2), 0, s, j));
+  else if (plan.rows <= 64) TXP_CUDA(launch(paged_join_kernel<T, D, 32>, dim3(borders, row_groups), dim3(D * 2), 0, s, j));
+  else TXP_CUDA(launch(paged_join_kernel<T, D, 0>, dim3(borders, (row_groups * (D / 16) + 7) / 8), dim3(256), 0, s, j));
   return TXD_OK;
 }
 

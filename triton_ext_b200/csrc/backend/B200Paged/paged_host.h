@@ -35,4 +35,21 @@ int shift_of(int page_size);  // log2
       return txp::fail(TXD_ERR_CUDA, "%s failed: %s", #expr, cudaGetErrorString(e_));             \
   } while (0)
 
+// The programmatic attribute lets a kernel be scheduled while its predecessor drains; every kernel launched with it waits
+// for its predecessor (griddepcontrol.wait) before it touches memory.
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const A &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace txp

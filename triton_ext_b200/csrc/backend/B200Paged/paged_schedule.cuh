@@ -329,105 +329,110 @@ struct JoinParams {
   int32_t ctas, rows, heads, head_dim;
 };
 
-// The joined value of a row: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, part by part.
+// The joined value of 16 columns of a row: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
 struct Joined {
   float acc[16], top, sum;
+  __device__ __forceinline__ void clear() {
+    top = -INFINITY;
+    sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  }
+  __device__ __forceinline__ void scale_to(float m) {  // a common reference of this and what comes next
+    const float next = fmaxf(top, m);
+    if (next == top) return;
+    const float f = fast_exp2(top - next);
+    top = next;
+    sum *= f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] *= f;
+  }
 };
 
-template <int D>
-__device__ __forceinline__ Joined join_parts(const JoinParams &p, int c, int first, int step, int parts, int row, int col) {
+// The parts of a tile are those of consecutive CTAs; the block of a tile's first border does the tile. A thread joins 16
+// columns of a row (32 bytes of output, a whole sector), the threads of a warp are rows, which the parts are laid out for.
+// What it costs is loads that wait for one another, so a warp takes 32 borders at once, and the loads of several parts are
+// under way together.
+// kRows (16 or 32: the rows of the streaming kernel's tiles; single tokens may have a few dozen parts): a block has a tile,
+// a warp 16 of its columns, and at 16 rows the half-warps take every second part. 0 (256 rows, two or three parts): a warp
+// has 32 rows and 16 columns, bound by reading them. (A thread that walked borders and parts one after another: 12 to 16 us
+// of 2 x 131071 or 64 ragged single tokens; all eight warps of a block on 16 columns: 8 us.)
+template <typename T, int D, int kRows>
+__global__ void __launch_bounds__(kRows ? D * 2 : 256) paged_join_kernel(const __grid_constant__ JoinParams p) {
+  constexpr int kColGroups = D / 16, kAtOnce = kRows ? 4 : 2, kSplit = kRows == 16 ? 2 : 1;
+  const int c = static_cast<int>(blockIdx.x) + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int unit = kRows ? static_cast<int>(blockIdx.y) * kColGroups + warp : static_cast<int>(blockIdx.y) * 8 + warp;
+  const int row = unit / kColGroups * 32 + (kRows == 16 ? lane & 15 : lane), col = unit % kColGroups * 16;
+  grid_dep_wait();
+  // lane i: the border that CTA c - 1 + i starts at, so part i of the tile that is cut there
+  int4 at = make_int4(-1, 0, 0, 0);
+  if (c - 1 + lane < p.ctas) at = p.borders[c - 1 + lane];
+  const int b = __shfl_sync(0xffffffffu, at.x, 1), h = __shfl_sync(0xffffffffu, at.y, 1), tile = __shfl_sync(0xffffffffu, at.z, 1);
+  uint32_t same = __ballot_sync(0xffffffffu, at.x == b && at.y == h && at.z == tile);
+  if (b < 0 || (same & 1u)) return;  // no tile is cut here, or it has been cut before
+  uint32_t there = __ballot_sync(0xffffffffu, at.w > 0) | 1u;  // an empty stretch has left nothing
+  const SeqInfo q = seq_info(p.s, b);
+  const int t0 = tile * p.s.tile_tokens, t1 = min(t0 + p.s.tile_tokens, q.q);
+  const int rows = (t1 - t0) * p.s.group;
+  if (unit / kColGroups * 32 >= rows || col >= p.head_dim) return;  // for the whole warp
+  same |= 1u;
   Joined j;
-  j.top = -INFINITY;
-  j.sum = 0.f;
+  j.clear();
+  for (int base = 0;; base += 32) {
+    const int run = same == 0xffffffffu ? 32 : __ffs(~same) - 1;  // parts base .. base + run - 1
+    for (int i = kSplit == 2 ? lane >> 4 : 0; i < run; i += kSplit * kAtOnce) {
+      float2 ml[kAtOnce];
+      float4 x[kAtOnce][4];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) j.acc[e] = 0.f;
-  auto slot = [&](int i) { return static_cast<long long>(c - 1 + i) * 2 + (i == 0 ? 1 : 0); };
-  auto there = [&](int i) { return i == 0 || p.borders[c - 1 + i].w > 0; };  // an empty stretch has left nothing
-#pragma unroll 4
-  for (int i = first; i < parts; i += step)
-    if (there(i)) j.top = fmaxf(j.top, p.ml[slot(i) * p.rows + row].x);
-  const float ref = j.top == -INFINITY ? 0.f : j.top;
-#pragma unroll 2
-  for (int i = first; i < parts; i += step) {
-    if (!there(i)) continue;
-    const float2 ml = p.ml[slot(i) * p.rows + row];
-    const float4 *o = p.part + (slot(i) * (D / 4) + col / 4) * p.rows + row;
-    float4 x[4];
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int k = i + u * kSplit;
+        ml[u] = make_float2(-INFINITY, 0.f);
+        if (k < run && (there >> k & 1u) && row < rows) {
+          const long long slot = (static_cast<long long>(c - 1 + base) + k) * 2 + (base + k == 0 ? 1 : 0);
+          ml[u] = p.ml[slot * p.rows + row];
+          const float4 *o = p.part + (slot * (D / 4) + col / 4) * p.rows + row;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = o[static_cast<long long>(e) * p.rows];
-    if (ml.x != -INFINITY) {  // a part that saw nothing has left no output
-      const float w = fast_exp2(ml.x - ref);
-      j.sum += w * ml.y;
+          for (int e = 0; e < 4; ++e) x[u][e] = o[static_cast<long long>(e) * p.rows];
+        }
+      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        j.acc[4 * e] += w * x[e].x;
-        j.acc[4 * e + 1] += w * x[e].y;
-        j.acc[4 * e + 2] += w * x[e].z;
-        j.acc[4 * e + 3] += w * x[e].w;
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (ml[u].x == -INFINITY) continue;  // nothing there, or nothing seen: no output was left
+        j.scale_to(ml[u].x);
+        const float w = fast_exp2(ml[u].x - j.top);
+        j.sum += w * ml[u].y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          j.acc[4 * e] += w * x[u][e].x;
+          j.acc[4 * e + 1] += w * x[u][e].y;
+          j.acc[4 * e + 2] += w * x[u][e].z;
+          j.acc[4 * e + 3] += w * x[u][e].w;
+        }
       }
     }
+    if (run < 32) break;
+    at = make_int4(-1, 0, 0, 0);
+    const int k = c - 1 + base + 32 + lane;
+    if (k < p.ctas) at = p.borders[k];
+    same = __ballot_sync(0xffffffffu, at.x == b && at.y == h && at.z == tile);
+    there = __ballot_sync(0xffffffffu, at.w > 0);
   }
-  return j;
-}
-
-// The parts of a tile are those of consecutive CTAs; the blocks of a tile's first border do the tile. A thread joins 16
-// columns of one row (32 bytes of output, a whole sector), a warp's threads are 32 rows, which the parts are laid out for.
-// kFewRows (single tokens: up to a few dozen parts, 16 to 64 rows): the 8 warps of a block share a tile's parts, because
-// one thread after another part's loads is what takes the time there (2 x 131071 tokens: 112 us with a thread for all
-// parts, 98); else (256 rows, two or three parts) a warp does all of them, bound by reading them.
-template <typename T, int D, bool kFewRows>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ JoinParams p) {
-  constexpr int kColGroups = D / 16;
-  __shared__ float s_acc[kFewRows ? 8 : 1][18][32];
-  grid_dep_wait();
-  const int c = static_cast<int>(blockIdx.x) + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int4 cut = p.borders[c], prev = p.borders[c - 1];
-  if (cut.x < 0 || (prev.x == cut.x && prev.y == cut.y && prev.z == cut.z)) return;
-  const SeqInfo q = seq_info(p.s, cut.x);
-  const int t0 = cut.z * p.s.tile_tokens, t1 = min(t0 + p.s.tile_tokens, q.q);
-  const int rows = (t1 - t0) * p.s.group;
-  const int unit = kFewRows ? blockIdx.y : blockIdx.y * 8 + warp;
-  const int row = unit / kColGroups * 32 + lane, col = unit % kColGroups * 16;
-  if (unit / kColGroups * 32 >= rows || col >= p.head_dim) return;  // for a whole warp, and block where they share
-  int parts = 2;  // of CTAs c - 1 and c, and of those behind whose border lies in the tile as well
-  for (bool more = true; more;) {
-    const int k = c + parts - 1 + lane;
-    int4 x = make_int4(-1, 0, 0, 0);
-    if (k < p.ctas) x = p.borders[k];
-    const uint32_t in = __ballot_sync(0xffffffffu, x.x == cut.x && x.y == cut.y && x.z == cut.z);
-    const int run = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
-    parts += run;
-    more = run == 32;
-  }
-  Joined j;
-  if (kFewRows) {
-    if (row < rows) {
-      j = join_parts<D>(p, c, warp, 8, parts, row, col);
+  if (kSplit == 2) {  // the other half-warp's parts; both halves come to the same
+    const float m = __shfl_xor_sync(0xffffffffu, j.top, 16);
+    const float next = fmaxf(j.top, m), ref = next == -INFINITY ? 0.f : next;
+    const float f = fast_exp2(j.top - ref);
+    j.top = next;
+    j.sum *= f;
+    j.sum += __shfl_xor_sync(0xffffffffu, j.sum, 16);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s_acc[warp][e][lane] = j.acc[e];
-      s_acc[warp][16][lane] = j.top;
-      s_acc[warp][17][lane] = j.sum;
+    for (int e = 0; e < 16; ++e) {
+      j.acc[e] *= f;
+      j.acc[e] += __shfl_xor_sync(0xffffffffu, j.acc[e], 16);
     }
-    __syncthreads();
-    if (warp > 0 || row >= rows) return;
-    const int n = min(parts, 8);
-    for (int w = 1; w < n; ++w) j.top = fmaxf(j.top, s_acc[w][16][lane]);
-    const float ref = j.top == -INFINITY ? 0.f : j.top;
-    j.sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) j.acc[e] = 0.f;
-    for (int w = 0; w < n; ++w) {
-      const float f = fast_exp2(s_acc[w][16][lane] - ref);
-      j.sum += f * s_acc[w][17][lane];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) j.acc[e] += f * s_acc[w][e][lane];
-    }
-  } else {
-    if (row >= rows) return;
-    j = join_parts<D>(p, c, 0, 1, parts, row, col);
   }
+  if (row >= rows || (kSplit == 2 && lane >= 16)) return;
   const float inv = j.sum > 0.f ? 1.f / j.sum : 0.f;
-  const int tok = q.q0 + t0 + row / p.s.group, head = cut.y * p.s.group + row % p.s.group;
+  const int tok = q.q0 + t0 + row / p.s.group, head = h * p.s.group + row % p.s.group;
   struct alignas(16) Eight { T x[8]; } y[2];
 #pragma unroll
   for (int e = 0; e < 16; ++e) y[e / 8].x[e % 8] = static_cast<T>(j.acc[e] * inv);  // rounded once, to nearest

@@ -10,8 +10,11 @@
 #pragma once
 
 #include "paged_host.h"
+#include "sm100_ptx.cuh"
 
 namespace txp {
+
+using namespace txd;
 
 struct PagesParams {
   uint4 *k, *v;
@@ -27,6 +30,7 @@ constexpr int kPlanPairs = 4;
 constexpr int kPlanThreads = 1024;
 
 __global__ void __launch_bounds__(256) pages_free_kernel(const __grid_constant__ PagesParams p, const int32_t *rows) {
+  grid_dep_wait();
   const int row = rows[blockIdx.x];
   if (row < 0 || row >= p.rows) {
     if (threadIdx.x == 0) atomicOr(p.status, kBadRow);
@@ -56,6 +60,7 @@ __device__ __forceinline__ bool fork_listed_later(const int32_t *dst, int n, int
 
 __global__ void __launch_bounds__(256) pages_fork_take_kernel(const __grid_constant__ PagesParams p, const int32_t *dst,
                                                               const int32_t *src, int n) {
+  grid_dep_wait();
   const int i = blockIdx.x;
   const int to = dst[i], from = src[i];
   int32_t *keep = p.ws + kPlanPairs + static_cast<long long>(i) * (p.width + 1);
@@ -79,6 +84,7 @@ __global__ void __launch_bounds__(256) pages_fork_take_kernel(const __grid_const
 }
 
 __global__ void __launch_bounds__(256) pages_fork_put_kernel(const __grid_constant__ PagesParams p, const int32_t *dst) {
+  grid_dep_wait();
   const int32_t *keep = p.ws + kPlanPairs + static_cast<long long>(blockIdx.x) * (p.width + 1);
   const int len = keep[p.width];
   if (len < 0) return;
@@ -128,30 +134,38 @@ __device__ __forceinline__ void load_refs(const PagesParams &p, int first, int (
   }
 }
 
-// Dynamic shared memory: end[n], last[n] (last page of the row if it is partly filled, else -1), seen[rows / 32].
+// Dynamic shared memory: end[n], last[n] (last page of the row if it is partly filled, else -1), row[n], len[n],
+// seen[rows / 32]. What takes the time is loads that wait for one another, so each is made once and the first step's
+// reference counts are loaded before anything else.
+constexpr int kFreshShared = 2048;  // free pages that are handed on in shared memory
+
 __global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan_kernel(const __grid_constant__ PagesParams p,
                                                                           const int32_t *rows, const int32_t *counts, int n) {
   extern __shared__ int32_t plan_smem[];
-  __shared__ int warp_sums[32];
+  __shared__ int warp_sums[32], s_fresh[kFreshShared];
   __shared__ int s_bad, s_pairs;
-  int32_t *end = plan_smem, *last = plan_smem + n;
-  uint32_t *seen = reinterpret_cast<uint32_t *>(plan_smem + 2 * n);
+  int32_t *end = plan_smem, *last = plan_smem + n, *s_row = plan_smem + 2 * n, *s_len = plan_smem + 3 * n;
+  uint32_t *seen = reinterpret_cast<uint32_t *>(plan_smem + 4 * n);
   int32_t *pairs = p.ws + kPlanPairs, *fresh = pairs + 2 * n;
   const int tid = threadIdx.x;
   const int slots = 1 << p.page_shift;
   if (tid == 0) s_bad = 0, s_pairs = 0;
   for (int i = tid; i < (p.rows + 31) / 32; i += kPlanThreads) seen[i] = 0;
+  grid_dep_wait();
+  int r0[16];
+  load_refs(p, tid * 16, r0);
   __syncthreads();
   for (int i = tid; i < n; i += kPlanThreads) {
     const int row = rows[i], count = counts[i];
-    int need = 0, page = -1;
+    int need = 0, page = -1, len_now = 0;
     uint32_t bad = 0;
     if (row < 0 || row >= p.rows || count < 0 || (atomicOr(&seen[row >> 5], 1u << (row & 31)) >> (row & 31) & 1u)) {
       bad = kBadRow;
     } else {
-      const long long len = max(p.lens[row], 0), want = (len + count + slots - 1) >> p.page_shift;
+      len_now = p.lens[row];
+      const long long len = max(len_now, 0), want = (len + count + slots - 1) >> p.page_shift;
       const long long have = (len + slots - 1) >> p.page_shift;
-      if (p.lens[row] < 0) {
+      if (len_now < 0) {
         bad = kBadLength;
       } else if (want > p.width || len + count > INT32_MAX) {
         bad = kNoRoomInRow;
@@ -166,6 +180,8 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan_kernel(const 
     if (bad) atomicOr(&s_bad, static_cast<int>(bad));
     end[i] = need;
     last[i] = page;
+    s_row[i] = row;
+    s_len[i] = len_now;
   }
   __syncthreads();
   // a shared last page is copied by its holder i if somebody holds it after those listed before i have left it
@@ -196,17 +212,18 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan_kernel(const 
     if (!copy) last[i] = -1;  // from here on: the page to copy
   }
   // the first need_all free pages, ascending
+  const bool shared = need_all <= kFreshShared;
   int found = 0;
   for (int base = 0; base < p.num_pages && found < need_all; base += kPlanThreads * 16) {
-    int r[16], zeros = 0, total;
-    load_refs(p, base + tid * 16, r);
+    if (base) load_refs(p, base + tid * 16, r0);
+    int zeros = 0, total;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) zeros += r[i] == 0;
+    for (int i = 0; i < 16; ++i) zeros += r0[i] == 0;
     int at = found + block_scan(zeros, &total, warp_sums);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (r[i] == 0) {
-        if (at < need_all) fresh[at] = base + tid * 16 + i;
+      if (r0[i] == 0) {
+        if (at < need_all) (shared ? s_fresh : fresh)[at] = base + tid * 16 + i;
         ++at;
       }
     found += total;
@@ -226,10 +243,10 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan_kernel(const 
       if (end[mid] > r) hi = mid;
       else lo = mid + 1;
     }
-    const int row = rows[lo], page = fresh[r];
+    const int page = (shared ? s_fresh : fresh)[r];
     const int off = r - (lo ? end[lo - 1] : 0), copy = last[lo] >= 0;
-    const int have = static_cast<int>((static_cast<long long>(p.lens[row]) + slots - 1) >> p.page_shift);
-    p.table[static_cast<long long>(row) * p.width + have + off - copy] = page;
+    const int have = static_cast<int>((static_cast<long long>(s_len[lo]) + slots - 1) >> p.page_shift);
+    p.table[static_cast<long long>(s_row[lo]) * p.width + have + off - copy] = page;
     p.refs[page] = 1;
     if (copy && off == 0) {
       const int slot = atomicAdd(&s_pairs, 1);
@@ -238,8 +255,8 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan_kernel(const 
       atomicSub(&p.refs[last[lo]], 1);
     }
   }
+  for (int i = tid; i < n; i += kPlanThreads) p.lens[s_row[i]] = s_len[i] + counts[i];
   __syncthreads();
-  for (int i = tid; i < n; i += kPlanThreads) p.lens[rows[i]] += counts[i];
   if (tid == 0) p.ws[0] = s_pairs;
 }
 
@@ -269,6 +286,7 @@ __device__ __forceinline__ void copy_pages(const PagesParams &p, const int32_t *
 }
 
 __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__ PagesParams p) {
+  grid_dep_wait();
   copy_pages(p, p.ws + kPlanPairs, p.ws[0]);
 }
 
@@ -279,6 +297,7 @@ struct ParamPairs {
 };
 __global__ void __launch_bounds__(256) pages_copy_listed_kernel(const __grid_constant__ PagesParams p,
                                                                 const __grid_constant__ ParamPairs pairs, int count) {
+  grid_dep_wait();
   copy_pages(p, pairs.pair, count);
 }
 
@@ -288,9 +307,10 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const 
   __shared__ int warp_sums[32];
   const int tid = threadIdx.x;
   int32_t *pairs = p.ws + kPlanPairs, *went = pairs + p.num_pages + 1;
-  int used = 0;
-  for (int base = 0; base < p.num_pages; base += kPlanThreads * 16) {
-    int r[16];
+  constexpr int kStep = kPlanThreads * 16;
+  grid_dep_wait();
+  int r[16], used = 0;
+  for (int base = 0; base < p.num_pages; base += kStep) {
     load_refs(p, base + tid * 16, r);
 #pragma unroll
     for (int i = 0; i < 16; ++i) used += r[i] > 0;
@@ -298,29 +318,27 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const 
   int live;
   block_scan(used, &live, warp_sums);
   int holes = 0, movers = 0;
-  for (int base = 0; base < p.num_pages; base += kPlanThreads * 16) {
-    int r[16], mine = 0, total;
+  for (int base = 0; base < p.num_pages; base += kStep) {
     const int first = base + tid * 16;
-    load_refs(p, first, r);
-    // a block-wide step of 16 K pages can hold the border: holes below it and movers above are counted in one sum each
+    if (p.num_pages > kStep) load_refs(p, first, r);  // a single step's counts are still here
+    // holes below the border, used pages above it: a step has at most 16384 of either, so both fit one sum
+    int mine = 0, total;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mine += first + i < live && r[i] == 0;
-    int at = holes + block_scan(mine, &total, warp_sums);
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (first + i < live && r[i] == 0) pairs[2 * at++ + 1] = first + i;
-    holes += total;
-    mine = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mine += first + i >= live && r[i] > 0;
-    at = movers + block_scan(mine, &total, warp_sums);
+    for (int i = 0; i < 16; ++i) mine += first + i < live ? (r[i] == 0) : (r[i] > 0) << 16;
+    const int before = block_scan(mine, &total, warp_sums);
+    int hole = holes + (before & 0xffff), mover = movers + (before >> 16);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      if (first + i < live || first + i >= p.num_pages) continue;
-      if (r[i] > 0) pairs[2 * at++] = first + i;
-      went[first + i] = first + i;
+      const int page = first + i;
+      if (page < live) {
+        if (r[i] == 0) pairs[2 * hole++ + 1] = page;
+      } else if (page < p.num_pages) {
+        if (r[i] > 0) pairs[2 * mover++] = page;
+        went[page] = page;
+      }
     }
-    movers += total;
+    holes += total & 0xffff;
+    movers += total >> 16;
   }
   __syncthreads();
   for (int i = tid; i < holes; i += kPlanThreads) {
@@ -336,6 +354,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const 
 }
 
 __global__ void __launch_bounds__(256) pages_compact_move_kernel(const __grid_constant__ PagesParams p) {
+  grid_dep_wait();
   const int32_t *pairs = p.ws + kPlanPairs, *went = pairs + p.num_pages + 1;
   const int count = p.ws[0], live = p.ws[1];
   if (!count) return;
