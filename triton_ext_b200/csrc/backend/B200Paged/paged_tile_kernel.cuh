@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     for (bool more = walk.start(p.s, &sched), last = false; !last; more = more && walk.next(p.s, &sched), ++count) {
       last = !more;
       const uint32_t i = count % kItems;
-      if (!warp_mbar_poll(smem_u32(&ctl.item_empty[i]), ((count / kItems) & 1u) ^ 1u, ac, kTimeout, lane)) break;
+      if (!warp_mbar_wait(smem_u32(&ctl.item_empty[i]), ((count / kItems) & 1u) ^ 1u, ac, kTimeout, lane)) break;
       if (lane == 0) {
         TileItem x = {};
         if (more) {
@@ -226,8 +226,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         if (cur < 0 || cur >= p.num_pages) atomicOr(p.s.status, kBadPage);
       };
       check();
-      // All lanes walk the copies of a tile together, one issues (with one copy a lane, the warp went through them one by one
-      // with everything of a copy set up anew: no faster, and 16 copies at 16-token pages)
+      // All lanes walk the copies of a tile together and one issues them; what a copy needs is at hand before the wait for its
+      // slot, because at D = 128 the ring's three slots leave a load little time.
       auto load_tile = [&](int j, bool is_v) {
         const int tok0 = (w.block + j) * 128;
         const int want = (tok0 >> p.page_shift) >> 5;
@@ -245,20 +245,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const uint32_t bar = smem_u32(&ctl.kv_full[slot]);
         const CUtensorMap *map = is_v ? &p.tmap_v : &p.tmap_k;
         const uint32_t dst = kv_addr0 + slot * tile_bytes;
+        const uint32_t bytes = (b1 - b0) * kAtoms * box_bytes;
+        const int in_mask = (1 << p.page_shift) - 1;
+        int id = __shfl_sync(0xffffffffu, ids, ((tok0 + (b0 << p.box_shift)) >> p.page_shift) & 31);
         if (!warp_mbar_poll(smem_u32(&ctl.kv_empty[slot]), ((issued / kStages) & 1u) ^ 1u, ac, kTimeout, lane)) {
           ok = false;
           return;
         }
-        if (issuer) mbar_arrive_expect_tx(bar, (b1 - b0) * kAtoms * box_bytes);
-        for (int b = b0; b < b1; ++b) {
+        if (issuer) mbar_arrive_expect_tx(bar, bytes);
+        for (int b = b0;;) {
           const int tok = tok0 + (b << p.box_shift);
-          const int id = __shfl_sync(0xffffffffu, ids, (tok >> p.page_shift) & 31);
-          const int in_page = tok & ((1 << p.page_shift) - 1);
           if (issuer) {
 #pragma unroll
             for (int a = 0; a < kAtoms; ++a)
-              tma_load_5d(dst + a * kAtomBytes + b * box_bytes, map, 0, in_page, a, w.head, id, bar);
+              tma_load_5d(dst + a * kAtomBytes + b * box_bytes, map, 0, tok & in_mask, a, w.head, id, bar);
           }
+          if (++b >= b1) break;
+          id = __shfl_sync(0xffffffffu, ids, ((tok0 + (b << p.box_shift)) >> p.page_shift) & 31);
         }
         __syncwarp();
         ++issued;
@@ -301,12 +304,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       ++taken;
       return slot;
     };
-    // A V tile: its rows that nobody sees are zeroed before they are multiplied.
+    // A V tile: its rows that nobody sees are zeroed before they are multiplied (only a tile's first and last block have any).
+    int fix_first = -1, fix_last = -1;
     auto take_v = [&](int j) -> uint32_t {
       const uint32_t slot = take();
-      const int tok0 = (w.block + j) * 128;
-      const int a = max(w.lo - tok0, 0), b = min(w.hi - tok0, 128);
-      if (ok && (a > 0 || b < 128)) {
+      if (ok && (j == fix_first || j == fix_last)) {
+        const int tok0 = (w.block + j) * 128;
+        const int a = max(w.lo - tok0, 0), b = min(w.hi - tok0, 128);
         for (int at = 0; at < kAtoms; ++at) {
           const uint32_t base = kv_addr0 + slot * tile_bytes + at * kAtomBytes;
           for (int i = lane; i < a * 8; i += 32) st_shared_v4(base + i * 16, 0u, 0u, 0u, 0u);
@@ -360,6 +364,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       const int nb = w.blocks;
       if (nb <= 0) continue;
       const int n_blk[2] = {nb, w.tokens > p.sub_tokens ? nb : 0};
+      fix_first = w.block * 128 < w.lo ? 0 : -1;
+      fix_last = (w.block + nb) * 128 > w.hi ? nb - 1 : -1;
       // S of block j: after the accumulator's last S has been read into registers (one tile's last before the next one's first)
       auto next_s = [&](int t, int j, uint32_t k_slot) {
         if (j >= n_blk[t]) return;
@@ -463,9 +469,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       const int pos = w.pos0 + rel;
       const int hi_r = !valid ? 0 : p.s.causal ? pos + 1 : w.kv;
       const int lo_r = p.s.window ? pos + 1 - p.s.window : 0;
-      // blocks inside [inner_lo, inner_hi) are seen whole by every row: the loop's unmasked part
-      const int inner_hi = p.s.causal ? w.pos0 + t + 1 : w.kv;
-      const int inner_lo = p.s.window ? w.pos0 + w.tokens - p.s.window : 0;
+      // blocks [seen_lo, seen_hi) of the part are seen whole by every row: the loop's unmasked part
+      const int seen_hi = ((p.s.causal ? w.pos0 + t + 1 : w.kv) >> 7) - w.block;
+      const int seen_lo = ((p.s.window ? max(w.pos0 + w.tokens - p.s.window, 0) : 0) + 127 >> 7) - w.block;
       float m_i = -INFINITY, l_i = 0.f;
       for (int j = 0; j < n; ++j, ++count) {
         if (!warp_mbar_poll(smem_u32(&ctl.s_full[t]), count & 1u, ac, kTimeout, lane)) {
@@ -481,8 +487,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         tmem_ld_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(&ctl.s_free[t]));
-        const int col0 = (w.block + j) * 128;
-        if (col0 + 128 > inner_hi || col0 < inner_lo) {
+        if (j >= seen_hi || j < seen_lo) {
+          const int col0 = (w.block + j) * 128;
           // by one word of bits for 32 columns: a third of the instructions of two compares for each score, and what this
           // code takes is mostly its own fetching (12 prompts, of 150 to 1500 tokens: 112 us with compares, 102)
           const int hi = hi_r - col0, lo = lo_r - col0;

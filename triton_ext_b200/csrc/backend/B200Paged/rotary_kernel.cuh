@@ -21,7 +21,7 @@
 
 namespace txp {
 
-constexpr int kRotaryThreads = 256;
+constexpr int kRotaryThreads = 128;
 constexpr int kUnroll = 2;  // heads whose vectors a lane has in flight
 
 enum RotaryKind : int32_t { kTurn = 0, kTurnToPage = 1, kCopyToPage = 2 };
@@ -136,7 +136,7 @@ __device__ __forceinline__ int find_sequence(const int32_t *cu, int n, int t, in
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kRotaryThreads, 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, 8) rotary_kernel(const __grid_constant__ RotaryParams p) {
   // cosine and sine of pair k * V + i at [i][k]: the lanes of a head read neighbouring banks
   __shared__ float2 s_turn[kRotaryThreads / 32][TX_ROPE_MAX_PAIRS];
   float2 *turn = s_turn[threadIdx.x >> 5];
