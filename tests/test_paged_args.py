@@ -24,6 +24,7 @@ def test_turns_are_the_frequencies_to_64_bits():
     for w, t in zip(rope.frequencies, turns_of(rope)):
         assert abs(t / 2 ** 64 - w / (2 * math.pi)) <= w * 2.0 ** -52
     assert turns_of(rope)[32:] == (0,) * (R.MAX_PAIRS - 32)
+    assert turns_of(R.Rope(2, frequencies=[-0.25]))[0] == (1 << 64) - turns_of(R.Rope(2, frequencies=[0.25]))[0]
     # one radian in 2^-64 turns, from the digits of 1 / (2 pi)
     assert turns_of(R.Rope(2))[0] == round(2 ** 64 * Fraction("0.15915494309189533576888376337251436203445964574046"))
 
@@ -111,6 +112,34 @@ def test_c_view_checks(built_libs, change, text, code):
                         a["batch"], a["width"], a["pages"], a["page_size"], a["heads"], a["head_dim"], a["dtype"], 0)
     rc, message = c_append(view)
     assert rc == code and text in message
+
+
+def c_attention(view, pointers=(1 << 20, 1 << 20, 0), strides=(128, 64, 128, 64), tokens=3, heads=2, max_q=1, causal=1,
+                window=0, scale=0.125, ws=1 << 20, size=1 << 40):
+    lib = P._lib()
+    problem = P._ATTN.pack(*pointers, *strides, tokens, heads, max_q, causal, window, scale)
+    return lib.tx_paged_attention(view, problem, ws, size, None), lib.tx_paged_last_error().decode()
+
+
+def test_c_attention_checks(built_libs):
+    view = Built().view()
+    for kw, text in ((dict(tokens=-1), "tokens"), (dict(heads=3), "multiple of kv_heads"), (dict(heads=0), "q_heads"),
+                     (dict(heads=130), "at most 64"), (dict(max_q=0), "max_q"), (dict(window=-1), "window"),
+                     (dict(window=3, causal=0), "window"), (dict(scale=0.0), "sm_scale"), (dict(scale=math.nan), "sm_scale"),
+                     (dict(scale=math.inf), "sm_scale"), (dict(tokens=2), "one new token"), (dict(pointers=(0, 1 << 20, 0)), "null tensor"),
+                     (dict(pointers=(1 << 20, (1 << 20) + 8, 0)), "16-byte aligned"), (dict(strides=(124, 64, 128, 64)), "multiples of 16 bytes"),
+                     (dict(strides=(128, 0, 128, 64)), "positive")):
+        rc, message = c_attention(view, **kw)
+        assert rc in (B.TXD_ERR_INVALID, B.TXD_ERR_UNSUPPORTED) and text in message, (kw, rc, message)
+    if not torch.cuda.is_available():
+        assert c_attention(view)[0] == B.TXD_ERR_NO_DEVICE
+    none = Built().view(table=torch.zeros(0, 2, dtype=i32), lens=torch.ones(0, dtype=i32))
+    assert c_attention(none, tokens=0)[0] == B.TXD_OK
+    # the workspace grows with the rows of a tile, and is asked for without a device
+    lib = P._lib()
+    sizes = [lib.tx_paged_attention_workspace(view, P._ATTN.pack(1 << 20, 1 << 20, 0, 128, 64, 128, 64, 3, 2, q, 1, 0, 0.1))
+             for q in (1,)]
+    assert sizes[0] > 0
 
 
 def test_c_append_checks(built_libs):

@@ -208,6 +208,101 @@ def test_strided_q_and_out_and_rows_behind(P):
     assert torch.equal(got[:43], want[:43]) and bool((out[43:] == 3.0).all()) and bool((out[:, 1] == 3.0).all())
 
 
+def test_many_sequences_in_tiles(P):
+    """More sequences than a CTA has threads, prompts and single tokens mixed, on the kernel for many rows."""
+    rng = random.Random(3)
+    q = [rng.choice([0, 1, 1, 2, 40, 130]) for _ in range(400)]
+    kv = [n + rng.choice([0, 0, 5, 200]) for n in q]
+    Batch(q, kv, 2, 1, 64, 16, bf16, seed=20).compare(P, 0.125)
+
+
+def test_waves_of_whole_tiles(P):
+    """Several tiles for every SM, of unequal lengths: dealt out whole, the rest cut."""
+    Batch([700, 1300, 90, 2000], [700, 2500, 4000, 2000], 16, 4, 64, 32, bf16, seed=21).compare(P, 0.125)
+    Batch([512] * 10, [512] * 10, 32, 32, 64, 64, f16, seed=22).compare(P, 0.125)
+
+
+def test_table_and_lengths_that_are_views(P):
+    b = Batch([1, 1, 1], [300, 20, 77], 4, 2, 64, 16, bf16, seed=23)
+    want = b.run(P, 0.125)
+    wide = torch.full((6, b.table.shape[1] + 9), -5, dtype=i32, device="cuda")
+    wide[::2, 4:4 + b.table.shape[1]] = b.table
+    b.table = wide[::2, 4:4 + b.table.shape[1]]
+    assert torch.equal(b.run(P, 0.125), want)
+    e = b.q[:, :1].expand(3, 4, 64)                               # one query for all heads
+    b.q = e.contiguous()
+    want = b.run(P, 0.125)
+    b.q = e
+    assert torch.equal(b.run(P, 0.125), want)
+
+
+def test_tokens_before_and_behind_the_sequences(P):
+    """cu_q may start above zero and end before the last row: rows outside are left alone, by append too."""
+    b = Batch([4, 40], [30, 300], 4, 2, 64, 16, bf16, seed=24)
+    want = b.run(P, 0.125)
+    q = torch.cat((b.q[:3], b.q, b.q[:2]))
+    out = torch.full_like(q, 9.0)
+    P.paged_attention(q, *b.pools, b.table, b.kv_lens, 0.125, cu_q=b.cu_q + 3, max_q=40, out=out)
+    assert torch.equal(out[3:47], want) and bool((out[:3] == 9.0).all()) and bool((out[47:] == 9.0).all())
+    pools = [x.clone() for x in b.pools]
+    k, v = (torch.full((49, 2, 64), x, dtype=bf16, device="cuda") for x in (2.0, 3.0))
+    got = torch.full_like(q, 9.0)
+    P.append(q, k, v, *pools, b.table, b.kv_lens, cu_q=b.cu_q + 3, out=got)
+    P.check()
+    assert torch.equal(got[3:47], b.q) and bool((got[:3] == 9.0).all()) and bool((got[47:] == 9.0).all())
+    expected = [x.clone() for x in b.pools]
+    for i, (n, m) in enumerate(zip(b.q_lens, b.kv_lens_host)):
+        pos = torch.arange(m - n, m, device="cuda")
+        for pool, value in zip(expected, (2.0, 3.0)):
+            pool[b.table[i].long()[pos // 16], pos % 16] = value
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(pools, expected))
+
+
+def test_in_place(P):
+    for q, kv in (([1] * 4, [3000, 5, 64, 900]), ([300, 70], [900, 70])):
+        b = Batch(q, kv, 8, 2, 128, 16, bf16, seed=25)
+        want = b.run(P, 0.09)
+        got = b.run(P, 0.09, out=b.q)
+        assert got.data_ptr() == b.q.data_ptr() and torch.equal(got, want)
+
+
+def test_pools_past_2_to_the_32_bytes_and_elements(P):
+    """Pages whose offsets pass 2^31 elements: append writes them, both kernels read them, a fork's copy moves them."""
+    page, hk, d = 256, 8, 128
+    pages = (1 << 31) // (page * hk * d) + 40                     # 8232 pages: 2.16e9 elements a pool
+    cache = P.PagedCache.create(pages, page, hk, d, rows=3, width=4)
+    cache.refs[: pages - 12] = 1                                  # only the last pages are free
+    g = torch.Generator().manual_seed(26)
+    lens = [600, 300]
+    cache.reserve(ints([0, 1]), ints(lens))
+    assert int(cache.table[0, 0]) == pages - 12
+    total = sum(lens)
+    q, k, v = (torch.randn(total, n, d, generator=g).to(bf16).cuda() for n in (16, hk, hk))
+    cu = ints([0, 600, 900])
+    table, kv = cache.table[:2], cache.lens[:2]
+    P.append(None, k, v, cache.k[0], cache.v[0], table, kv, cu_q=cu)
+    cache.fork(ints([2]), ints([0]))
+    cache.reserve(ints([2]), ints([1]))
+    P.check()
+    kk, vv = (torch.cat((x[:600], x[:1])) for x in (k, v))
+    P.append(None, kk[600:], vv[600:], cache.k[0], cache.v[0], cache.table[2:], cache.lens[2:])
+    many = P.paged_attention(q, cache.k[0], cache.v[0], table, kv, 0.09, cu_q=cu, max_q=600)
+    one = P.paged_attention(q[:1], cache.k[0], cache.v[0], cache.table[2:], cache.lens[2:], 0.09)
+    P.check()
+
+    def dense(q, k, v, causal):
+        s = torch.einsum("thd,khd->htk", q.double(), k.double().repeat_interleave(2, 1)) * 0.09
+        if causal:
+            s = s.masked_fill(torch.ones(s.shape[1:], device="cuda").triu(1).bool(), -math.inf)
+        return torch.einsum("htk,khd->thd", s.softmax(-1), v.double().repeat_interleave(2, 1))
+
+    # values of standard deviation 1, |o| and the weighted magnitudes below 5: 2^-8 * 5 for the output's rounding and as
+    # much for P's
+    for got, want in ((many[:600], dense(q[:600], k[:600], v[:600], True)), (many[600:], dense(q[600:], k[600:], v[600:], True)),
+                      (one, dense(q[:1], kk, vv, False))):
+        assert float((got.double() - want).abs().max()) <= 2 * 5 * 2.0 ** -8
+
+
 @pytest.mark.parametrize("max_q", [1, 5, 4096])
 def test_max_q_only_chooses_the_kernel(P, max_q):
     Batch([5, 77], [300, 900], 8, 2, 128, 16, bf16, seed=10).compare(P, 0.09, max_q=max_q)

@@ -70,8 +70,8 @@ int check_view(const tx_paged_view *c, tx_paged_view *out) {
     if (extent[i] == 1) out->k_stride[i] = out->v_stride[i] = c->head_dim;
   c = out;
   for (int i = 0; i < 3; ++i)
-    if (c->k_stride[i] < 0 || c->v_stride[i] < 0 || c->k_stride[i] % 8 || c->v_stride[i] % 8)
-      return fail(TXD_ERR_UNSUPPORTED, "cache strides must be non-negative multiples of 16 bytes");
+    if (c->k_stride[i] < 1 || c->v_stride[i] < 1 || c->k_stride[i] % 8 || c->v_stride[i] % 8)
+      return fail(TXD_ERR_UNSUPPORTED, "cache strides must be positive multiples of 16 bytes");
   if (c->batch > 0 && (!c->table || !c->kv_lens)) return fail(TXD_ERR_INVALID, "null table or kv_lens");
   if (c->table_stride < 0) return fail(TXD_ERR_INVALID, "negative table stride");
   return TXD_OK;

@@ -242,8 +242,8 @@ int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_problem *
     const bool one = (i == 0 ? pr->tokens : pr->q_heads) == 1;
     q_stride[i] = one ? plan.view.head_dim : pr->q_stride[i];
     o_stride[i] = one ? plan.view.head_dim : pr->out_stride[i];
-    if (q_stride[i] < 0 || o_stride[i] < 0 || q_stride[i] % 8 || o_stride[i] % 8)
-      return fail(TXD_ERR_UNSUPPORTED, "strides of q and out must be non-negative multiples of 16 bytes");
+    if (q_stride[i] < 1 || o_stride[i] < 1 || q_stride[i] % 8 || o_stride[i] % 8)
+      return fail(TXD_ERR_UNSUPPORTED, "strides of q and out must be positive multiples of 16 bytes");
   }
   uint32_t *status = nullptr;
   if ((rc = device_ready(&status))) return rc;

@@ -163,6 +163,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if d != k_pages.shape[3]:
         _invalid(f"q has head_dim {d}, the cache {k_pages.shape[3]}")
     qs = _token_strides(q, "q", tokens, d, k_pages)
+    if 0 in qs:  # expanded heads or tokens
+        q = q.contiguous()
+        qs = q.stride()
     if cu_q is None:
         if tokens != page_table.shape[0]:
             _invalid(f"without cu_q there is one new token for each of the {page_table.shape[0]} sequences, got {tokens}")
