@@ -63,16 +63,17 @@ int encode_queries(CUtensorMap *map, const void *ptr, const tx_paged_view &c, co
   return TXD_OK;
 }
 
-struct RowShape {  // rows a CTA attends with, and CTAs per SM
-  int mt, ks, per_sm;
+constexpr int kRowBlock32 = 128;  // KV tokens of a block where a tile has 32 rows
+
+// Which kernel takes a call of few rows: a function of the group, the bound on a sequence's new tokens and the head dimension.
+struct RowShape {
+  int rows, block, per_sm;  // rows of a tile, KV tokens of a block, CTAs per SM
 };
 
-// Which kernel takes a call: a function of the group, the bound on a sequence's new tokens and the head dimension.
-RowShape row_shape(int kernel_d, int group, int max_q) {
-  const long long rows = static_cast<long long>(group) * (max_q > 0 ? max_q : 1);
-  if (rows <= 16) return {1, 4, kernel_d == 256 ? 1 : 2};
-  if (rows <= 32) return {2, 4, 1};
-  return {4, 2, 1};  // head dimension 256 only
+RowShape row_shape(int kernel_d, long long rows) {
+  if (kernel_d == 256) return {rows <= 16 ? 16 : rows <= 32 ? 32 : 64, 64, 1};
+  if (rows <= 16) return {16, 64, 2};
+  return {32, kRowBlock32, 1};
 }
 
 int sm_count() {
@@ -116,12 +117,12 @@ int make_plan(const tx_paged_view *cache, const tx_paged_attn_problem *pr, Plan 
   plan->kernel_d = c.head_dim <= 64 ? 64 : c.head_dim;
   int max_q = pr->max_q;
   if (max_q > pr->tokens) max_q = pr->tokens;
-  plan->shape = row_shape(plan->kernel_d, plan->group, max_q);
+  plan->shape = row_shape(plan->kernel_d, static_cast<long long>(plan->group) * (max_q > 0 ? max_q : 1));
   // 128-row tiles on tcgen05 for head dimensions up to 128 (256 columns of O for two sub-tiles do not fit tensor memory
   // next to S); up to 32 rows the streaming kernel. Measured, 16 sequences of up to 4100 tokens, 32 + 8 heads of 128, tiles
   // against streams: 32 rows 71 us and 57, 64 rows 66 us and 84.
   plan->tiled = plan->kernel_d <= 128 && static_cast<long long>(plan->group) * max_q > 32;
-  plan->rows = plan->tiled ? 256 : plan->shape.mt * 16;
+  plan->rows = plan->tiled ? 256 : plan->shape.rows;
   plan->ctas = sm_count() * (plan->tiled ? 1 : plan->shape.per_sm);
   plan->borders_bytes = (static_cast<size_t>(plan->ctas) * 16 + 255) / 256 * 256;
   const size_t rows = static_cast<size_t>(plan->ctas) * 2 * plan->rows;
@@ -142,31 +143,30 @@ cudaError_t allow_smem(void (*kernel)(P), int bytes, std::atomic<uint64_t> *done
   return e;
 }
 
-template <bool kBf16, int D, int MT, int KS, int kStages, int kPerSm>
+template <bool kBf16, int D, int BS, int MT, int KS, int kStages, int kPerSm>
 int launch_row(const RowParams &prm, int ctas, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  auto kernel = paged_row_kernel<kBf16, D, MT, KS, kStages, kPerSm>;
-  constexpr int smem = row_smem_bytes<D, kStages>();
+  auto kernel = paged_row_kernel<kBf16, D, BS, MT, KS, kStages, kPerSm>;
+  constexpr int smem = row_smem_bytes<D, BS, kStages>();
   TXP_CUDA(allow_smem(kernel, smem, &done));
   TXP_CUDA(launch(kernel, dim3(ctas), dim3((MT * KS + 1) * 32), smem, stream, prm));
   return TXD_OK;
 }
 
 template <bool kBf16>
-int launch_row_any(const Plan &plan, const RowParams &prm, cudaStream_t s) {
-  const int mt = plan.shape.mt;
-  // ring: 96 KB a CTA where two share an SM, up to 192 KB where one has it
-  if (plan.kernel_d == 64) {
-    if (mt == 1) return launch_row<kBf16, 64, 1, 4, 6, 2>(prm, plan.ctas, s);
-    return launch_row<kBf16, 64, 2, 4, 8, 1>(prm, plan.ctas, s);
+int launch_row_any(const RowShape &shape, int kernel_d, const RowParams &prm, int ctas, cudaStream_t s) {
+  // ring: 96 KB a CTA where two share an SM, 192 KB where one has it
+  if (kernel_d == 64) {
+    if (shape.rows == 16) return launch_row<kBf16, 64, 64, 1, 4, 6, 2>(prm, ctas, s);
+    return launch_row<kBf16, 64, kRowBlock32, 2, 4, 768 / kRowBlock32, 1>(prm, ctas, s);
   }
-  if (plan.kernel_d == 128) {
-    if (mt == 1) return launch_row<kBf16, 128, 1, 4, 3, 2>(prm, plan.ctas, s);
-    return launch_row<kBf16, 128, 2, 4, 6, 1>(prm, plan.ctas, s);
+  if (kernel_d == 128) {
+    if (shape.rows == 16) return launch_row<kBf16, 128, 64, 1, 4, 3, 2>(prm, ctas, s);
+    return launch_row<kBf16, 128, kRowBlock32, 2, 4, 384 / kRowBlock32, 1>(prm, ctas, s);
   }
-  if (mt == 1) return launch_row<kBf16, 256, 1, 4, 3, 1>(prm, plan.ctas, s);
-  if (mt == 2) return launch_row<kBf16, 256, 2, 4, 3, 1>(prm, plan.ctas, s);
-  return launch_row<kBf16, 256, 4, 2, 3, 1>(prm, plan.ctas, s);
+  if (shape.rows == 16) return launch_row<kBf16, 256, 64, 1, 4, 3, 1>(prm, ctas, s);
+  if (shape.rows == 32) return launch_row<kBf16, 256, 64, 2, 4, 3, 1>(prm, ctas, s);
+  return launch_row<kBf16, 256, 64, 4, 2, 3, 1>(prm, ctas, s);
 }
 
 template <bool kBf16, int D>
@@ -263,7 +263,7 @@ int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_problem *
   sched.causal = pr->causal ? 1 : 0;
   sched.window = pr->window > (1 << 30) ? 1 << 30 : pr->window;
   sched.max_kv = c.table_width * c.page_size;
-  sched.block_shift = 6;
+  sched.block_shift = shift_of(plan.shape.block);
   sched.tile_cost = 2;
   sched.min_part = 2;
   sched.min_share = 3;
@@ -316,14 +316,15 @@ int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_problem *
     if ((rc = bf16 ? launch_tile_any<true>(plan, prm, stream) : launch_tile_any<false>(plan, prm, stream))) return rc;
   } else {
     RowParams prm = {};
-    const int box_rows = c.page_size < 64 ? c.page_size : 64;
+    const int box_rows = c.page_size < plan.shape.block ? c.page_size : plan.shape.block;
     const int groups = plan.kernel_d / 64;
     if ((rc = encode_pool(&prm.tmap_k, c.k, c, c.k_stride, box_rows, groups))) return rc;
     if ((rc = encode_pool(&prm.tmap_v, c.v, c, c.v_stride, box_rows, groups))) return rc;
     fill(prm, box_rows);
     prm.q = pr->q;
     for (int i = 0; i < 2; ++i) prm.q_stride[i] = q_stride[i];
-    if ((rc = bf16 ? launch_row_any<true>(plan, prm, stream) : launch_row_any<false>(plan, prm, stream))) return rc;
+    if ((rc = bf16 ? launch_row_any<true>(plan.shape, plan.kernel_d, prm, plan.ctas, stream)
+                   : launch_row_any<false>(plan.shape, plan.kernel_d, prm, plan.ctas, stream))) return rc;
   }
 
   JoinParams join = {};

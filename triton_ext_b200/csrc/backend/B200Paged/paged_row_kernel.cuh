@@ -1,6 +1,6 @@
 // Paged attention for few rows (single tokens, drafted tokens): bound by reading K and V once from HBM.
 //
-// A CTA walks its stretch of the work line (paged_schedule.cuh). One warp streams KV blocks of 64 tokens through a ring in
+// A CTA walks its stretch of the work line (paged_schedule.cuh). One warp walks it and streams KV blocks of BS tokens through a ring in
 // shared memory by TMA, one copy per page and tensor (page coordinate from the page table, so a bad entry reads zeros); the
 // other warps are MT groups of 16 rows x KS shares of a block's tokens. Each keeps a running maximum, a running sum and its
 // output in registers through the whole tile (one pass over the keys), on m16n8k16 tensor instructions: at 16 rows per
@@ -20,7 +20,19 @@
 
 namespace txp {
 
-constexpr int kRowBlock = 64;  // KV tokens of a block
+constexpr int kRowItems = 4;   // tiles that the producer may be ahead
+
+// One tile of a CTA's work, as the consumers take it.
+struct RowItem {
+  int tok0, tokens;   // new tokens [tok0, tok0 + tokens) of the batch
+  int pos0;           // position of the first in its sequence
+  int head;
+  int lo, hi, kv;     // keys that some row sees: [lo, hi); the sequence's keys
+  int first_key;      // of the first block of this part
+  int blocks;
+  int whole, slot;    // not a part of a cut tile; else the place of the partial result
+  int more;           // 0: the work is done
+};
 
 struct RowParams {
   CUtensorMap tmap_k, tmap_v;  // {64 columns, slots, column groups, heads, pages}
@@ -36,7 +48,7 @@ struct RowParams {
   float2 *ml;
   unsigned long long wait_limit_ns;
   float qk_scale;  // sm_scale * log2(e)
-  int32_t num_pages, page_shift, box_shift;  // box: rows of one TMA copy, min(page_size, 64)
+  int32_t num_pages, page_shift, box_shift;  // box: rows of one TMA copy, min(page_size, BS)
   int32_t heads, head_dim;
   int32_t inject_stall;
 };
@@ -75,25 +87,43 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *m, 
       : "memory");
 }
 
-template <int D, int kStages>
-constexpr int row_smem_bytes() { return kStages * 2 * kRowBlock * D * 2 + 1024; }
+// Whether it holds for any of kThreads threads, which meet at named barrier 1.
+template <int kThreads>
+__device__ __forceinline__ bool any_of(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.u32 p, %1, 0;\n"
+      "bar.red.or.pred q, 1, %2, p;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(r)
+      : "r"(x ? 1u : 0u), "n"(kThreads)
+      : "memory");
+  return r != 0;
+}
 
-template <bool kBf16, int D, int MT, int KS, int kStages, int kBlocksPerSm>
+template <int D, int BS, int kStages>
+constexpr int row_smem_bytes() { return kStages * 2 * BS * D * 2 + 1024; }
+
+template <bool kBf16, int D, int BS, int MT, int KS, int kStages, int kBlocksPerSm>
 __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_kernel(const __grid_constant__ RowParams p) {
   constexpr int kConsumers = MT * KS;
   constexpr int kThreads = (kConsumers + 1) * 32;
-  constexpr int kTok = kRowBlock / KS;      // tokens of a block that one warp takes
+  constexpr int kTok = BS / KS;             // tokens of a block that one warp takes
   constexpr int kSlabs = kTok / 16;
   constexpr int kGroups = D / 64;           // column groups of 128 bytes
-  constexpr uint32_t kTensorBytes = kRowBlock * D * 2;
+  constexpr uint32_t kTensorBytes = BS * D * 2;
   constexpr uint32_t kStageBytes = 2 * kTensorBytes;
-  constexpr int kRounds = MT * KS / 4;      // of the join: a ring slot holds 4 * 16 rows of D fp32 values
+  constexpr int kRounds = MT * KS * 16 / BS;  // of the join: a ring slot holds BS rows of D fp32 values
   constexpr int kJoinCols = D / kRounds;
   static_assert(kJoinCols >= 32, "a round has whole groups of columns");
 
   extern __shared__ uint8_t row_smem_raw[];
   __shared__ SchedSmem sched;
-  __shared__ uint64_t full[kStages], empty[kStages];
+  __shared__ uint64_t full[kStages], empty[kStages], item_full[kRowItems], item_empty[kRowItems];
+  __shared__ RowItem items[kRowItems];
   __shared__ float2 s_ml[KS][MT * 16];
   __shared__ uint32_t abort_flag;
   const uint32_t ring = (smem_u32(row_smem_raw) + 1023u) & ~1023u;
@@ -103,6 +133,10 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&full[i]), 1);
       mbar_init(smem_u32(&empty[i]), kConsumers);
+    }
+    for (int i = 0; i < kRowItems; ++i) {
+      mbar_init(smem_u32(&item_full[i]), 1);
+      mbar_init(smem_u32(&item_empty[i]), kConsumers);
     }
     abort_flag = 0;
     fence_mbar_init();
@@ -117,21 +151,50 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
   ac.flag = &abort_flag;
   ac.status = p.s.status;
   ac.limit_ns = p.wait_limit_ns;
-  Walk w;
 
   if (warp == kConsumers) {
-    // ------------------------------ producer ------------------------------
-    uint32_t issued = 0;
+    // ------------------------------ producer: walks the work, hands the tiles on, loads their blocks ------------------------------
+    Walk w;
+    uint32_t issued = 0, count = 0;
     bool ok = true;
-    const int boxes = kRowBlock >> p.box_shift;           // copies of a tensor per block
+    const int boxes = BS >> p.box_shift;           // copies of a tensor per block
     const uint32_t box_bytes = (128u << p.box_shift) * kGroups;
+    auto hand_on = [&](bool more) {
+      const uint32_t i = count % kRowItems;
+      if (!warp_mbar_poll(smem_u32(&item_empty[i]), ((count / kRowItems) & 1u) ^ 1u, ac, kTimeout, lane)) {
+        ok = false;
+        return;
+      }
+      if (lane == 0) {
+        RowItem x = {};
+        if (more) {
+          x.tok0 = w.q.q0 + w.t.t0;
+          x.tokens = w.t.t1 - w.t.t0;
+          x.pos0 = w.t.off + w.t.t0;
+          x.head = w.at.h;
+          x.lo = w.t.lo;
+          x.hi = w.t.hi;
+          x.kv = w.q.kv;
+          x.first_key = (w.t.blk0 + w.from) * BS;
+          x.blocks = w.to - w.from;
+          x.whole = w.whole();
+          x.slot = static_cast<int>(w.slot());
+          x.more = 1;
+        }
+        items[i] = x;
+        mbar_arrive(smem_u32(&item_full[i]));
+      }
+      __syncwarp();
+      ++count;
+    };
     for (bool more = w.start(p.s, &sched); more && ok; more = w.next(p.s, &sched)) {
+      hand_on(true);
       const int32_t *row = p.table + w.at.b * p.table_stride;
       const int first_page = w.t.lo >> p.page_shift, last_page = (w.t.hi - 1) >> p.page_shift;
       int window = -1, page_reg = 0;  // 32 entries of the page table, one a lane
       for (int j = w.from; j < w.to && ok; ++j) {
         const uint32_t slot = issued % kStages, pass = issued / kStages;
-        const int tok0 = (w.t.blk0 + j) * kRowBlock;
+        const int tok0 = (w.t.blk0 + j) * BS;
         // lane: tensor (K first) and box
         const int box = lane < boxes ? lane : lane - boxes;
         const int tok = tok0 + (box << p.box_shift), page = tok >> p.page_shift;
@@ -167,6 +230,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
         ++issued;
       }
     }
+    if (ok) hand_on(false);
     if (!ok) {  // copies in flight land before the shared memory goes away
       if (lane == 0)
         for (uint32_t i = issued > kStages ? issued - kStages : 0u; i < issued; ++i) {
@@ -182,8 +246,8 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
     const int mt = warp / KS, ks = warp % KS;
     const int g4 = lane >> 2, l4 = lane & 3;
     uint32_t taken = 0;
-    // After a wait that ran out a warp goes on without waiting, so that every warp still meets the others at the
-    // barriers below; what it computes then is reported as undefined.
+    // After a wait that ran out a warp goes through the tile's end without waiting, so that every warp still meets the
+    // others at the barriers below; what it computes then is reported as undefined.
     bool ok = true;
     auto take = [&]() -> uint32_t {
       const uint32_t slot = taken % kStages;
@@ -208,42 +272,49 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
     const uint32_t k_row = ((lane >> 4) * 8 + x7) * 128u, k_chunk = (lane >> 3) & 1;
     const uint32_t v_row = (((lane >> 3) & 1) * 8 + x7) * 128u, v_chunk = lane >> 4;
 
-    for (bool more = w.start(p.s, &sched); more; more = w.next(p.s, &sched)) {
-      const int rows = (w.t.t1 - w.t.t0) * p.s.group;
+    for (uint32_t count = 0;; ++count) {
+      const uint32_t item = count % kRowItems;
+      if (ok && !warp_mbar_poll(smem_u32(&item_full[item]), (count / kRowItems) & 1u, ac, kTimeout, lane)) ok = false;
+      if (any_of<kConsumers * 32>(!ok)) break;  // all of them leave, or none
+      const RowItem w = items[item];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&item_empty[item]));
+      if (!w.more) break;
+      const int rows = w.tokens * p.s.group;
       // ---- Q: the A fragments of this warp's 16 rows, straight from memory ----
       uint32_t qf[D / 16][4];
       int hi_r[2], lo_r[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = mt * 16 + g4 + e * 8;
-        const int tok = w.t.t0 + r / p.s.group;
-        const int head = w.at.h * p.s.group + r % p.s.group;
+        const int tok = r / p.s.group;
+        const int head = w.head * p.s.group + r % p.s.group;
         const bool valid = r < rows;
-        const T *src = static_cast<const T *>(p.q) + (w.q.q0 + tok) * p.q_stride[0] + head * p.q_stride[1] + l4 * 2;
+        const T *src = static_cast<const T *>(p.q) + (w.tok0 + tok) * p.q_stride[0] + head * p.q_stride[1] + l4 * 2;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const bool in = valid && (D > 64 || kk * 16 < p.head_dim);
           qf[kk][e] = in ? *reinterpret_cast<const uint32_t *>(src + kk * 16) : 0u;
           qf[kk][2 + e] = in ? *reinterpret_cast<const uint32_t *>(src + kk * 16 + 8) : 0u;
         }
-        const int pos = w.t.off + tok;
-        hi_r[e] = !valid ? 0 : p.s.causal ? min(pos + 1, w.q.kv) : w.q.kv;
+        const int pos = w.pos0 + tok;
+        hi_r[e] = !valid ? 0 : p.s.causal ? pos + 1 : w.kv;
         lo_r[e] = p.s.window ? max(pos + 1 - p.s.window, 0) : 0;
       }
       // blocks outside [inner_lo, inner_hi) have keys that some row of the tile does not see
-      const int inner_hi = p.s.causal ? w.t.off + w.t.t0 + 1 : w.q.kv;
-      const int inner_lo = p.s.window ? w.t.off + w.t.t1 - p.s.window : 0;
+      const int inner_hi = p.s.causal ? w.pos0 + 1 : w.kv;
+      const int inner_lo = p.s.window ? w.pos0 + w.tokens - p.s.window : 0;
       float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 
-      for (int j = w.from; j < w.to; ++j) {
+      for (int j = 0; j < w.blocks; ++j) {
         const uint32_t slot = take();
         const uint32_t k_base = ring + slot * kStageBytes, v_base = k_base + kTensorBytes;
-        const int blk_tok = (w.t.blk0 + j) * kRowBlock;
-        const bool edge = blk_tok + kRowBlock > inner_hi || blk_tok < inner_lo;
+        const int blk_tok = w.first_key + j * BS;
+        const bool edge = blk_tok + BS > inner_hi || blk_tok < inner_lo;
         // ---- S = Q K^T ----
         float s[kSlabs * 2][4];
 #pragma unroll
@@ -265,10 +336,10 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
 #pragma unroll
           for (int i = 0; i < kSlabs; ++i) {
             const int key = blk_tok + ks * kTok + i * 16;
-            if (key >= w.t.lo && key + 16 <= w.t.hi) continue;
+            if (key >= w.lo && key + 16 <= w.hi) continue;
             for (int x = lane; x < 16 * 8 * kGroups; x += 32) {
               const int tok = (x >> 3) & 15;
-              if (key + tok < w.t.lo || key + tok >= w.t.hi)
+              if (key + tok < w.lo || key + tok >= w.hi)
                 st_shared_v4(v_base + slab[i] + (x >> 7) * group_bytes + tok * 128u + (x & 7) * 16u, 0u, 0u, 0u, 0u);
             }
           }
@@ -339,7 +410,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
       }
 
       // ---- the tile's end: the KS warps of each row group become one ----
-      const bool any = w.to > w.from;
+      const bool any = w.blocks > 0;
       if (any) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -361,7 +432,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
         for (int i = 0; i < KS; ++i) top = fmaxf(top, s_ml[i][mt * 16 + g4 + e * 8].x);
         f[e] = top == -INFINITY ? 0.f : fast_exp2(m[e] - top);
       }
-      const bool whole = w.whole();
+      const bool whole = w.whole != 0;
 #pragma unroll 1
       for (int round = 0; round < kRounds; ++round) {
         // rows are kJoinCols fp32 values; groups of 8 columns are exchanged by the row's last bits against bank conflicts
@@ -405,15 +476,15 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
           }
           if (whole) {
             const float inv = sum > 0.f ? 1.f / sum : 0.f;
-            const int tok = w.q.q0 + w.t.t0 + r / p.s.group, head = w.at.h * p.s.group + r % p.s.group;
+            const int tok = w.tok0 + r / p.s.group, head = w.head * p.s.group + r % p.s.group;
             if (col < p.head_dim) {
               T *dst = static_cast<T *>(p.out) + tok * p.out_stride[0] + head * p.out_stride[1] + col;
               *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<kBf16>(x.x * inv, x.y * inv), pack2<kBf16>(x.z * inv, x.w * inv));
             }
             if (p.m_out && col == 0) p.m_out[static_cast<long long>(tok) * p.heads + head] = sum > 0.f ? top + log2f(sum) : -INFINITY;
           } else {
-            p.part[(w.slot() * (D / 4) + col / 4) * (MT * 16) + r] = x;
-            if (col == 0) p.ml[w.slot() * (MT * 16) + r] = make_float2(top, sum);
+            p.part[(static_cast<long long>(w.slot) * (D / 4) + col / 4) * (MT * 16) + r] = x;
+            if (col == 0) p.ml[static_cast<long long>(w.slot) * (MT * 16) + r] = make_float2(top, sum);
           }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
