@@ -102,10 +102,16 @@ __device__ __forceinline__ void next_tile(const Sched &s, Cut &c, SeqInfo &q) {
 
 __device__ __forceinline__ bool same_tile(const Cut &a, const Cut &b) { return a.b == b.b && a.h == b.h && a.i == b.i; }
 
+// Quotient of non-negative numbers, by the short division where both are short.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
 // The place at distance r along the tiles of sequence b, moved to a tile's start where a part would be too short.
 __device__ __forceinline__ Cut resolve(const Sched &s, int b, long long distance, long long per_head) {
   SeqInfo q = seq_info(s, b);
-  const int h = static_cast<int>(distance / per_head);
+  const int h = static_cast<int>(quotient(distance, per_head));
   long long r = distance - h * per_head;
   Cut c = {b, h, 0, 0};
   TileInfo t = tile_info(s, q, 0);
@@ -198,20 +204,23 @@ __device__ __forceinline__ void find_work(const Sched &s, SchedSmem *sm, int4 *b
   }
   if (tid < kMaxWaves + 2) sm->cut[tid] = Cut{s.batch, 0, 0, 0};
   if (tid == 0) sm->waves = kMaxWaves, sm->x[0] = sm->x[1] = -1;
-  long long before[2] = {mine, tid < s.batch ? static_cast<long long>(tiles_of(s, q)) * s.kv_heads : 0}, totals[2];
-  block_scan<kThreads, 2>(before, totals, sm->sums);
+  constexpr int kSums = kWaves ? 2 : 1;
+  long long before[kSums], totals[kSums];
+  before[0] = mine;
+  if constexpr (kWaves) before[1] = tid < s.batch ? static_cast<long long>(tiles_of(s, q)) * s.kv_heads : 0;
+  block_scan<kThreads, kSums>(before, totals, sm->sums);
   const long long total = totals[0];
   long long skipped = 0;  // length of what is dealt out whole
   int waves = 0;
   long long dealt[2] = {0, 0}, dealt_all[2] = {0, 1};  // thread c: CTA c's whole tiles, and what is left for its stretch
-  if (kWaves && one_pass && n <= kThreads && totals[1] >= n && totals[1] < INT32_MAX) {
+  if constexpr (kWaves) if (one_pass && n <= kThreads && totals[1] >= n && totals[1] < INT32_MAX) {
     const SeqTable tab = {scratch, scratch + kThreads, scratch + 2 * kThreads};
     tab.tiles_before[tid] = static_cast<int>(before[1]);
     tab.q[tid] = q.q;
     tab.kv[tid] = q.kv;
     __syncthreads();
     const int most = min(static_cast<int>(totals[1]) / n, s.waves);
-    const long long target = total / n;
+    const long long target = quotient(total, n);
     auto tile_of = [&](int f) { return tile_at(s, tab, f * n + ((f & 1) ? n - 1 - tid : tid)); };
     // only as many waves as no CTA's whole tiles alone are more than its share of the work
     int fit = 0;
@@ -243,7 +252,7 @@ __device__ __forceinline__ void find_work(const Sched &s, SchedSmem *sm, int4 *b
       sm->x[tid - cta] = skipped + static_cast<long long>(static_cast<double>(rest) * (static_cast<double>(dealt[1]) / static_cast<double>(dealt_all[1])));
     if (tid == cta && cta == n - 1) sm->x[1] = total;
   } else if (tid < 2 && cta < parts && rest > 0) {
-    sm->x[tid] = skipped + rest * (cta + tid) / parts;
+    sm->x[tid] = skipped + quotient(rest * (cta + tid), parts);
   }
   if (tid == 0) sm->waves = waves;
   __syncthreads();
