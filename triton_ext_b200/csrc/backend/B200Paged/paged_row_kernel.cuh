@@ -8,7 +8,10 @@
 // their softmax. At a tile's end the KS warps of a row group are joined through a ring slot that the producer leaves empty.
 //
 // The share of a tile that HBM has to deliver is all there is to wait for: the ring holds 96 KB a CTA, two CTAs an SM
-// (at 16 rows), which covers HBM's latency several times.
+// (at 16 rows), which covers HBM's latency several times. 64 ragged sequences of up to 8192 tokens, 32 + 8 heads of 128:
+// 212 us, 6.4 TB/s. At 32 rows a warp's own chain (products, exponentials, products) is as long as its share of the bytes
+// takes, about 0.9 us for 16 tokens, so a warp takes 32 tokens at a time there (8 drafted tokens over up to 4100: 51 us with
+// 16, 47 with 32). Short calls are latency: 2.2 us to share the work out, 2 to 3 us to the first block, 2.5 us to join.
 #pragma once
 
 #include <cuda_bf16.h>

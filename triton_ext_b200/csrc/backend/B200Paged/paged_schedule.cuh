@@ -5,7 +5,7 @@
 // Few long tiles (a single sequence over a long cache, a batch of single tokens): the line is cut into n equal stretches, one
 // a CTA. Many tiles: the first F * n are dealt out whole, wave by wave, every second wave in reverse, so that the CTAs that
 // run at the same time are at neighbouring tiles and share their keys and values through L2 (all CTAs on contiguous
-// stretches took 4.74 ms for 32 heads of 16384 tokens of 128, this 3.92: every head's keys were in use at once); the
+// stretches took 4.74 ms for 32 heads of 16384 tokens of 128, this 3.85: every head's keys were in use at once); the
 // rest of the line is cut so that all CTAs come to the same length. Either way a CTA has at most two parts of tiles:
 // those leave their unnormalised output, maximum and sum in the workspace, and a second kernel joins them in order.
 // Nothing waits for another CTA, nothing is counted with atomics, and the order of every sum depends on the lengths alone.
