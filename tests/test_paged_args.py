@@ -67,7 +67,7 @@ class Built:
     def view(self, **kw):
         a = dict(k=self.k, v=self.v, table=self.table, lens=self.lens, cu=None)
         a.update(kw)
-        return P._view(a["k"], a["v"], a["table"], a["lens"], a["cu"], torch.device("cpu"))
+        return P._view(a["k"], a["v"], a["table"], a["lens"], a["cu"], -1)[0]
 
 
 def status_of(call):

@@ -97,10 +97,8 @@ int launch_rotary_t(const RotaryParams &prm, int v, cudaStream_t stream) {
   const long long warps = static_cast<long long>(prm.total) * prm.slices;
   const unsigned grid = static_cast<unsigned>((warps + kRotaryThreads / 32 - 1) / (kRotaryThreads / 32));
   constexpr int kWide = 16 / static_cast<int>(sizeof(T));
-  if (v == kWide) rotary_kernel<T, kWide><<<grid, kRotaryThreads, 0, stream>>>(prm);
-  else if (v >= 2) rotary_kernel<T, 2><<<grid, kRotaryThreads, 0, stream>>>(prm);
-  else rotary_kernel<T, 1><<<grid, kRotaryThreads, 0, stream>>>(prm);
-  TXP_CUDA(cudaGetLastError());
+  auto kernel = v == kWide ? rotary_kernel<T, kWide> : v >= 2 ? rotary_kernel<T, 2> : rotary_kernel<T, 1>;
+  TXP_CUDA(launch(kernel, dim3(grid), dim3(kRotaryThreads), 0, stream, prm));
   count_launches(1);
   return TXD_OK;
 }

@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 
 #include "paged_host.h"
+#include "sm100_ptx.cuh"
 
 namespace txp {
 
@@ -145,6 +146,7 @@ __global__ void __launch_bounds__(kRotaryThreads, 8) rotary_kernel(const __grid_
   const uint32_t id = blockIdx.x * (kRotaryThreads / 32) + (threadIdx.x >> 5);
   const uint32_t t = p.slices == 1 ? id : id / p.slices;
   if (t >= p.total) return;
+  txd::grid_dep_wait();
   const int slice = static_cast<int>(id - t * p.slices);
   const bool append = p.positions == nullptr;
   // ---- the token's position, and where an append puts it ----

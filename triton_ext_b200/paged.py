@@ -66,33 +66,41 @@ _STATE = struct.Struct("2Pq3P6i")
 
 
 def _view(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
-          cu_q: Optional[torch.Tensor], device: torch.device) -> bytes:
-    shape, dtype = k_pages.shape, _DTYPES.get(k_pages.dtype)
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != k_pages.dtype:
+          cu_q: Optional[torch.Tensor], device: int) -> tuple[bytes, int, int, int]:
+    """(the packed tx_paged_view, batch, kv_heads, head_dim); `device` as `Tensor.get_device` numbers it."""
+    dtype, code = k_pages.dtype, _DTYPES.get(k_pages.dtype)
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != dtype:
         _invalid("k_pages and v_pages must be [pages, page_size, kv_heads, head_dim] of one shape and type")
-    if dtype is None:
-        raise B.DotError(B.TXD_ERR_UNSUPPORTED, f"cache dtype {k_pages.dtype}: f16 and bf16 are built")
-    if not (k_pages.device == v_pages.device == page_table.device == kv_lens.device == device):
+    if code is None:
+        raise B.DotError(B.TXD_ERR_UNSUPPORTED, f"cache dtype {dtype}: f16 and bf16 are built")
+    if (k_pages.get_device() != device or v_pages.get_device() != device or page_table.get_device() != device or
+            kv_lens.get_device() != device):
         _invalid("the cache, page_table and kv_lens must be on the device of the new tokens")
-    ks, vs, ts = k_pages.stride(), v_pages.stride(), page_table.stride()
-    if ks[3] != 1 or vs[3] != 1:
+    pages, page_size, heads, d = shape
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    if k3 != 1 or v3 != 1:
         _invalid("head_dim must be the contiguous dimension of k_pages and v_pages")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or (ts[1] != 1 and page_table.shape[1] > 1):
+    table_shape, table_stride = page_table.shape, page_table.stride()
+    if page_table.dtype != torch.int32 or len(table_shape) != 2 or (table_stride[1] != 1 and table_shape[1] > 1):
         _invalid("page_table must be int32 [batch, pages of a sequence] with unit column stride")
-    batch, width = page_table.shape
-    if kv_lens.dtype != torch.int32 or kv_lens.dim() != 1 or kv_lens.shape[0] != batch or (batch > 1 and kv_lens.stride(0) != 1):
+    batch, width = table_shape
+    if kv_lens.dtype != torch.int32 or kv_lens.shape != (batch,) or (batch > 1 and kv_lens.stride(0) != 1):
         _invalid(f"kv_lens must be a contiguous int32 vector of {batch} lengths")
-    if cu_q is not None and (cu_q.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] != batch + 1 or
-                             (batch > 0 and cu_q.stride(0) != 1) or cu_q.device != device):
-        _invalid(f"cu_q must be a contiguous int32 vector of {batch + 1} offsets on the device of the new tokens")
-    return _VIEW.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], page_table.data_ptr(),
-                      ts[0], kv_lens.data_ptr(), cu_q.data_ptr() if cu_q is not None else 0, batch, width, shape[0], shape[1],
-                      shape[2], shape[3], dtype, 0)
+    cu = 0
+    if cu_q is not None:
+        if (cu_q.dtype != torch.int32 or cu_q.shape != (batch + 1,) or (batch > 0 and cu_q.stride(0) != 1) or
+                cu_q.get_device() != device):
+            _invalid(f"cu_q must be a contiguous int32 vector of {batch + 1} offsets on the device of the new tokens")
+        cu = cu_q.data_ptr()
+    return _VIEW.pack(k_pages.data_ptr(), v_pages.data_ptr(), k0, k1, k2, v0, v1, v2, page_table.data_ptr(), table_stride[0],
+                      kv_lens.data_ptr(), cu, batch, width, pages, page_size, heads, d, code, 0), batch, heads, d
 
 
-def _token_strides(x: torch.Tensor, name: str, tokens: int, head_dim: int, like: torch.Tensor) -> tuple[int, int]:
+def _token_strides(x: torch.Tensor, name: str, tokens: int, head_dim: int, like: torch.Tensor, device: int) -> tuple[int, int]:
     shape, s = x.shape, x.stride()
-    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim or x.dtype != like.dtype or x.device != like.device:
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim or x.dtype != like.dtype or x.get_device() != device:
         _invalid(f"{name} must be [tokens, heads, head_dim] = [{tokens}, *, {head_dim}] of the cache's type and device")
     if s[2] != 1 and head_dim > 1:
         _invalid(f"head_dim must be the contiguous dimension of {name}")
@@ -114,31 +122,36 @@ def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages:
     [batch], the sequences' lengths WITH the new tokens. cu_q: int32 [batch + 1], where each sequence's new tokens start
     (None: one token for each sequence, in order). Sequence b's new tokens take its last positions. out: where the turned q
     goes (q itself is allowed). Tokens behind cu_q[-1] are left alone: their rows of `out` are not written."""
-    lib = _lib()
-    if not k.is_cuda:
+    lib = _lib_cache or _lib()
+    device = k.get_device()
+    if device < 0:
         _not_cuda(k)
-    view = _view(k_pages, v_pages, page_table, kv_lens, cu_q, k.device)
-    tokens, heads, d = k.shape if k.dim() == 3 else _invalid("k must be [tokens, kv_heads, head_dim]")
-    if heads != k_pages.shape[2] or v.shape != k.shape or d != k_pages.shape[3]:
+    view, batch, kv_heads, d = _view(k_pages, v_pages, page_table, kv_lens, cu_q, device)
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != kv_heads or v.shape != shape or shape[2] != d:
         _invalid("k and v must be [tokens, kv_heads, head_dim] with the cache's heads and head_dim")
-    if cu_q is None and tokens != page_table.shape[0]:
-        _invalid(f"without cu_q there is one new token for each of the {page_table.shape[0]} sequences, got {tokens}")
-    ks, vs = _token_strides(k, "k", tokens, d, k_pages), _token_strides(v, "v", tokens, d, k_pages)
+    tokens = shape[0]
+    if cu_q is None and tokens != batch:
+        _invalid(f"without cu_q there is one new token for each of the {batch} sequences, got {tokens}")
+    ks, vs = _token_strides(k, "k", tokens, d, k_pages, device), _token_strides(v, "v", tokens, d, k_pages, device)
     q_ptr, o_ptr, q_heads, qs, os_ = 0, 0, 0, (0, 0), (0, 0)
     if q is not None:
-        qs, q_heads = _token_strides(q, "q", tokens, d, k_pages), q.shape[1]
+        qs, q_heads = _token_strides(q, "q", tokens, d, k_pages, device), q.shape[1]
         if out is None:
             out = torch.empty_like(q)
-        elif out.shape != q.shape or (tokens > 1 and out.stride(0) == 0) or (q_heads > 1 and out.stride(1) == 0):
-            _invalid("out must have the shape of q and not be an expanded tensor")
-        os_ = _token_strides(out, "out", tokens, d, k_pages)
+            os_ = out.stride()
+        else:
+            os_ = _token_strides(out, "out", tokens, d, k_pages, device)
+            if out.shape != q.shape or (tokens > 1 and os_[0] == 0) or (q_heads > 1 and os_[1] == 0):
+                _invalid("out must have the shape of q and not be an expanded tensor")
         q_ptr, o_ptr = q.data_ptr(), out.data_ptr()
     elif out is not None:
         _invalid("out is for the turned q: there is none")
     if rope is not None and rope.rotary_dim > d:
         _invalid(f"rotary_dim {rope.rotary_dim} exceeds head_dim {d}")
-    problem = _APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, *qs, *ks, *vs, *os_, tokens, q_heads)
-    _call(k.device, lib.tx_paged_append, view, rope._packed if rope is not None else None, problem)
+    problem = _APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1],
+                           tokens, q_heads)
+    _call(device, lib.tx_paged_append, view, rope._packed if rope is not None else None, problem)
     return out
 
 
@@ -154,32 +167,35 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     of them. max_q: a bound on the new tokens of one sequence, needed with cu_q. A row that sees nothing gives zeros.
     Returns the output, with `return_m` also [tokens, heads] fp32 of max + log2(sum) (base 2), -inf where nothing is seen.
     Rows behind cu_q[-1] are left alone."""
-    lib = _lib()
-    if not q.is_cuda:
+    lib = _lib_cache or _lib()
+    device = q.get_device()
+    if device < 0:
         _not_cuda(q)
-    device = q.device
-    view = _view(k_pages, v_pages, page_table, kv_lens, cu_q, device)
-    tokens, heads, d = q.shape if q.dim() == 3 else _invalid("q must be [tokens, heads, head_dim]")
-    if d != k_pages.shape[3]:
-        _invalid(f"q has head_dim {d}, the cache {k_pages.shape[3]}")
-    qs = _token_strides(q, "q", tokens, d, k_pages)
+    view, batch, _, head_dim = _view(k_pages, v_pages, page_table, kv_lens, cu_q, device)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != head_dim:
+        _invalid(f"q must be [tokens, heads, head_dim] with the cache's head_dim {head_dim}, got {tuple(shape)}")
+    tokens, heads, d = shape
+    qs = _token_strides(q, "q", tokens, d, k_pages, device)
     if 0 in qs:  # expanded heads or tokens
         q = q.contiguous()
         qs = q.stride()
     if cu_q is None:
-        if tokens != page_table.shape[0]:
-            _invalid(f"without cu_q there is one new token for each of the {page_table.shape[0]} sequences, got {tokens}")
+        if tokens != batch:
+            _invalid(f"without cu_q there is one new token for each of the {batch} sequences, got {tokens}")
         max_q = 1
     elif max_q is None:
         _invalid("cu_q needs max_q, a bound on the new tokens of one sequence")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or (tokens > 1 and out.stride(0) == 0) or (heads > 1 and out.stride(1) == 0):
-        _invalid("out must have the shape of q and not be an expanded tensor")
-    os_ = _token_strides(out, "out", tokens, d, k_pages)
-    m = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_m else None
+        os_ = out.stride()
+    else:
+        os_ = _token_strides(out, "out", tokens, d, k_pages, device)
+        if out.shape != shape or (tokens > 1 and os_[0] == 0) or (heads > 1 and os_[1] == 0):
+            _invalid("out must have the shape of q and not be an expanded tensor")
+    m = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_m else None
     problem = _ATTN.pack(q.data_ptr(), out.data_ptr(), m.data_ptr() if return_m else 0, qs[0], qs[1], os_[0], os_[1], tokens,
-                         heads, max_q, int(causal), window, sm_scale)
+                         heads, max_q, 1 if causal else 0, window, sm_scale)
     size = lib.tx_paged_attention_workspace(view, problem)
     ws = q.new_empty((size + 1) // 2)  # 16-bit values
     _call(device, lib.tx_paged_attention, view, problem, ws.data_ptr(), size)
@@ -239,7 +255,7 @@ class PagedCache:
     def free(self, rows: torch.Tensor) -> None:
         """Give the pages of the listed rows back (those that no other row holds become free) and empty the rows."""
         lib, rows = _lib(), self._list(rows, "rows")
-        _call(rows.device, lib.tx_pages_free, self._state, rows.data_ptr(), rows.shape[0])
+        _call(rows.get_device(), lib.tx_pages_free, self._state, rows.data_ptr(), rows.shape[0])
 
     def fork(self, dst: torch.Tensor, src: torch.Tensor) -> None:
         """Row dst[i] becomes what row src[i] was before the call, sharing its pages. Rows may be both (the reordering of a
@@ -247,7 +263,7 @@ class PagedCache:
         lib, dst = _lib(), self._list(dst, "dst")
         src = self._list(src, "src", dst.shape[0])
         ws = self._workspace(lib, dst)
-        _call(dst.device, lib.tx_pages_fork, self._state, dst.data_ptr(), src.data_ptr(), dst.shape[0], ws.data_ptr())
+        _call(dst.get_device(), lib.tx_pages_fork, self._state, dst.data_ptr(), src.data_ptr(), dst.shape[0], ws.data_ptr())
 
     def reserve(self, rows: torch.Tensor, counts: torch.Tensor) -> None:
         """Make room for counts[i] more tokens in row rows[i] and add them to its length, before they are appended. New pages
@@ -256,7 +272,7 @@ class PagedCache:
         lib, rows = _lib(), self._list(rows, "rows")
         counts = self._list(counts, "counts", rows.shape[0])
         ws = self._workspace(lib, rows)
-        _call(rows.device, lib.tx_pages_reserve, self._state, rows.data_ptr(), counts.data_ptr(), rows.shape[0], ws.data_ptr())
+        _call(rows.get_device(), lib.tx_pages_reserve, self._state, rows.data_ptr(), counts.data_ptr(), rows.shape[0], ws.data_ptr())
 
     def compact(self) -> None:
         """Move pages (all layers) so that the used ones are the lowest, the fewest that do it; the table follows."""
@@ -264,7 +280,7 @@ class PagedCache:
         if not self.k.is_cuda:
             _not_cuda(self.k)
         ws = self.refs.new_empty((lib.tx_pages_workspace(self._state, 0) + 3) // 4)
-        _call(self.k.device, lib.tx_pages_compact, self._state, ws.data_ptr())
+        _call(self.k.get_device(), lib.tx_pages_compact, self._state, ws.data_ptr())
 
     def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
         """Copy the contents of pages src[i] to dst[i] in every layer. Host lists; no page may be a destination twice, or
@@ -278,4 +294,4 @@ class PagedCache:
         for x in (*src, *dst):
             if not 0 <= int(x) < pages:
                 _invalid(f"page {x} is outside the {pages} pages")
-        _call(self.k.device, lib.tx_pages_copy, self._state, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n)
+        _call(self.k.get_device(), lib.tx_pages_copy, self._state, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n)

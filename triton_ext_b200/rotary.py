@@ -111,25 +111,25 @@ _PART = struct.Struct("2P6q2i")
 _NO_PART = _PART.pack(0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
-def _part(x: torch.Tensor, out: torch.Tensor) -> bytes:
-    a, b = x.stride(), out.stride()
-    return _PART.pack(x.data_ptr(), out.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], x.shape[1], 0)
-
-
-def _check_tensor(x: torch.Tensor, name: str) -> None:
-    if x.dim() != 4:
-        raise B.DotError(B.TXD_ERR_INVALID, f"{name} must be [Z, H, N_CTX, HEAD_DIM]")
-    if not x.is_cuda:
-        raise B.DotError(B.TXD_ERR_NO_DEVICE, f"{name} must be a CUDA tensor: there is no CPU path")
-
-
-def _check_out(out: Optional[torch.Tensor], x: torch.Tensor, name: str) -> None:
-    if out is None:
-        return
+def _check_out(out: torch.Tensor, x: torch.Tensor, name: str) -> None:
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
         raise B.DotError(B.TXD_ERR_INVALID, f"{name} must have its input's shape, type and device, HEAD_DIM contiguous")
     if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
         raise B.DotError(B.TXD_ERR_INVALID, f"{name} must not be an expanded tensor")
+
+
+def _part(x: torch.Tensor, out: Optional[torch.Tensor], heads: int, name: str) -> tuple[bytes, torch.Tensor]:
+    """The packed tx_rotary_part of x, and where its result goes."""
+    if out is not None:
+        _check_out(out, x, name)
+    a = x.stride()
+    if a[3] != 1:
+        x = x.contiguous()
+        a = x.stride()
+    if out is None:
+        out = torch.empty_like(x)
+    b = out.stride()
+    return _PART.pack(x.data_ptr(), out.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], heads, 0), out
 
 
 def rotary_forward(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rope: Rope, *, inverse: bool = False,
@@ -139,51 +139,45 @@ def rotary_forward(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.
     q, k: [Z, H, N_CTX, HEAD_DIM] of one 16-bit type or float32 and any strides with HEAD_DIM contiguous (others are
     copied); k may have its own number of heads. positions: int32 or int64, [N_CTX] or [Z, N_CTX]. out_q, out_k: where the
     results go (the inputs themselves are allowed: in place). inverse: turn backwards."""
-    lib = _lib()
-    _check_tensor(q, "q")
-    z, _, n, d = q.shape
-    if k is not None:
-        _check_tensor(k, "k")
-        if k.shape[0] != z or k.shape[2] != n or k.shape[3] != d or k.dtype != q.dtype or k.device != q.device:
-            raise B.DotError(B.TXD_ERR_INVALID, "q and k must agree in all but their heads, and in type and device")
+    lib = _lib_cache or _lib()
+    shape = q.shape
+    device = q.get_device()
+    if len(shape) != 4:
+        raise B.DotError(B.TXD_ERR_INVALID, "q must be [Z, H, N_CTX, HEAD_DIM]")
+    if device < 0:
+        raise B.DotError(B.TXD_ERR_NO_DEVICE, "q must be a CUDA tensor: there is no CPU path")
+    z, heads, n, d = shape
     dtype = _DTYPES.get(q.dtype)
     if dtype is None:
         raise B.DotError(B.TXD_ERR_UNSUPPORTED, f"rotary dtype {q.dtype}: f16, bf16 and f32 are built")
     if rope.rotary_dim > d:
         raise B.DotError(B.TXD_ERR_INVALID, f"rotary_dim {rope.rotary_dim} exceeds HEAD_DIM {d}")
-    if positions.device != q.device or positions.dtype not in (torch.int32, torch.int64):
+    wide = positions.dtype == torch.int64
+    if not (wide or positions.dtype == torch.int32) or positions.get_device() != device:
         raise B.DotError(B.TXD_ERR_INVALID, "positions must be int32 or int64 on the device of q")
-    if positions.dim() == 1 and positions.shape[0] == n:
-        pos_stride = (0, positions.stride(0))
-    elif positions.dim() == 2 and positions.shape[1] == n and positions.shape[0] == z:
-        pos_stride = positions.stride()
+    pos_shape, pos_stride = positions.shape, positions.stride()
+    if pos_shape == (n,):
+        pos_stride = (0, pos_stride[0])
+    elif pos_shape != (z, n):
+        raise B.DotError(B.TXD_ERR_INVALID, f"positions must be [{n}] or [{z}, {n}], got {tuple(pos_shape)}")
+    first, out_q = _part(q, out_q, heads, "out_q")
+    if k is None:
+        parts, second, out_k = 1, _NO_PART, None
     else:
-        raise B.DotError(B.TXD_ERR_INVALID, f"positions must be [{n}] or [{z}, {n}], got {tuple(positions.shape)}")
-    _check_out(out_q, q, "out_q")
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    if out_q is None:
-        out_q = torch.empty_like(q)
-    parts, second = 1, _NO_PART
-    if k is not None:
-        _check_out(out_k, k, "out_k")
-        if k.stride(3) != 1:
-            k = k.contiguous()
-        if out_k is None:
-            out_k = torch.empty_like(k)
-        parts, second = 2, _part(k, out_k)
-    packed = _HEAD.pack(z, n, d, dtype, int(inverse), int(positions.dtype == torch.int64), pos_stride[0], pos_stride[1],
-                        parts, 0) + _part(q, out_q) + second
-    _call(q.device, lib.tx_rotary, rope._packed, packed, positions.data_ptr())
-    return out_q, (out_k if k is not None else None)
+        ks = k.shape
+        if len(ks) != 4 or ks[0] != z or ks[2] != n or ks[3] != d or k.dtype != q.dtype or k.get_device() != device:
+            raise B.DotError(B.TXD_ERR_INVALID, "q and k must agree in all but their heads, and in type and device")
+        parts = 2
+        second, out_k = _part(k, out_k, ks[1], "out_k")
+    packed = _HEAD.pack(z, n, d, dtype, 1 if inverse else 0, 1 if wide else 0, pos_stride[0], pos_stride[1], parts, 0) + first + second
+    _call(device, lib.tx_rotary, rope._packed, packed, positions.data_ptr())
+    return out_q, out_k
 
 
-def _call(device: torch.device, function, *args) -> None:
-    """One C entry point on the current stream of a device (made the current device meanwhile); raises if it fails. The
+def _call(index: int, function, *args) -> None:
+    """One C entry point on the current stream of device `index` (made the current device meanwhile); raises if it fails. The
     stream is the entry point's last argument."""
-    index = device.index
-    before = torch.cuda.current_device()
-    if before == index:
+    if torch.cuda.current_device() == index:
         rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -228,7 +222,6 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
 def check(device=None) -> None:
     """Synchronise the current stream and raise for what the rotary, append, paged attention and page kernels found wrong
     on the device since the last check."""
-    dev = torch.device("cuda") if device is None else torch.device(device)
-    if dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
-    _call(dev, _lib().tx_paged_check)
+    index = None if device is None else device if isinstance(device, int) else torch.device(device).index
+    lib = _lib()
+    _call(torch.cuda.current_device() if index is None else index, lib.tx_paged_check)
