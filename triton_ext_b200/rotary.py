@@ -22,14 +22,14 @@ from . import backend as B
 MAX_PAIRS = 128
 _DTYPES = {torch.float16: B.TXD_F16, torch.bfloat16: B.TXD_BF16, torch.float32: B.TXD_F32}
 # 1 / (2 pi) to 100 binary digits: a product with an exact double gives all 64 bits of a turn's fraction
-_INV_2PI = Fraction(201752859139730814931732094791, 1 << 100)
+_INV_2PI_BITS = 201752859139730814931732094791
+_INV_2PI = Fraction(_INV_2PI_BITS, 1 << 100)
 
 
 def _turns(w: float) -> int:
     """w / (2 pi) as a 64-bit fraction of a turn, rounded to nearest."""
-    n, d = w.as_integer_ratio()
-    d <<= 100 - 64
-    return ((2 * n * _INV_2PI.numerator + d) // (2 * d)) & 0xFFFFFFFFFFFFFFFF
+    n, d = w.as_integer_ratio()  # d is a power of two
+    return (((n * _INV_2PI_BITS >> (d.bit_length() + 34)) + 1) >> 1) & 0xFFFFFFFFFFFFFFFF
 
 _lib_cache = None
 
