@@ -134,6 +134,21 @@ def test_strides_in_place_and_outputs(R):
     close(R.rotary_forward(m, None, pos, rope)[0], *turned64(m, pos, rope))
 
 
+def test_both_tensors_have_to_be_copied(R):
+    """Neither head dimension is contiguous: both copies have to live until the launch. The gradient of a sum is such a tensor
+    (its strides are zero)."""
+    rope, pos = R.Rope(64), torch.arange(50, device="cuda")
+    q, k = (torch.randn(2, 3, 64, 50, device="cuda").bfloat16().transpose(2, 3) for _ in range(2))
+    want = R.rotary_forward(q.contiguous(), None, pos, rope)[0], R.rotary_forward(k.contiguous(), None, pos, rope)[0]
+    got = R.rotary_forward(q, k, pos, rope)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q, k = (x.contiguous().requires_grad_() for x in (q, k))
+    a, b = R.rotary(q, k, pos, rope)
+    gq, gk = torch.autograd.grad(a.sum() + 2 * b.sum(), (q, k))
+    one = R.rotary_forward(torch.ones_like(q), None, pos, rope, inverse=True)[0]
+    assert torch.equal(gq, one) and torch.equal(gk, 2 * one)
+
+
 def test_empty(R):
     rope = R.Rope(32)
     q, k = tensor((2, 3, 0, 64), bf16, 1), tensor((2, 1, 0, 64), bf16, 1)

@@ -118,8 +118,9 @@ def _check_out(out: torch.Tensor, x: torch.Tensor, name: str) -> None:
         raise B.DotError(B.TXD_ERR_INVALID, f"{name} must not be an expanded tensor")
 
 
-def _part(x: torch.Tensor, out: Optional[torch.Tensor], heads: int, name: str) -> tuple[bytes, torch.Tensor]:
-    """The packed tx_rotary_part of x, and where its result goes."""
+def _part(x: torch.Tensor, out: Optional[torch.Tensor], heads: int, name: str):
+    """The packed tx_rotary_part of x, where its result goes, and what it is read from (x or a copy of it): to be kept until
+    the launch, or its memory may be the next copy's."""
     if out is not None:
         _check_out(out, x, name)
     a = x.stride()
@@ -129,7 +130,7 @@ def _part(x: torch.Tensor, out: Optional[torch.Tensor], heads: int, name: str) -
     if out is None:
         out = torch.empty_like(x)
     b = out.stride()
-    return _PART.pack(x.data_ptr(), out.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], heads, 0), out
+    return _PART.pack(x.data_ptr(), out.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], heads, 0), out, x
 
 
 def rotary_forward(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rope: Rope, *, inverse: bool = False,
@@ -160,7 +161,7 @@ def rotary_forward(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.
         pos_stride = (0, pos_stride[0])
     elif pos_shape != (z, n):
         raise B.DotError(B.TXD_ERR_INVALID, f"positions must be [{n}] or [{z}, {n}], got {tuple(pos_shape)}")
-    first, out_q = _part(q, out_q, heads, "out_q")
+    first, out_q, q = _part(q, out_q, heads, "out_q")
     if k is None:
         parts, second, out_k = 1, _NO_PART, None
     else:
@@ -168,7 +169,7 @@ def rotary_forward(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.
         if len(ks) != 4 or ks[0] != z or ks[2] != n or ks[3] != d or k.dtype != q.dtype or k.get_device() != device:
             raise B.DotError(B.TXD_ERR_INVALID, "q and k must agree in all but their heads, and in type and device")
         parts = 2
-        second, out_k = _part(k, out_k, ks[1], "out_k")
+        second, out_k, k = _part(k, out_k, ks[1], "out_k")
     packed = _HEAD.pack(z, n, d, dtype, 1 if inverse else 0, 1 if wide else 0, pos_stride[0], pos_stride[1], parts, 0) + first + second
     _call(device, lib.tx_rotary, rope._packed, packed, positions.data_ptr())
     return out_q, out_k
