@@ -290,6 +290,18 @@ def test_append(P, q_lens, kv_lens, h, hk, d, page, dtype, rd, inter, heads_firs
     assert again.data_ptr() == q.data_ptr() and torch.equal(q[:total], out[:total])
 
 
+def test_append_of_overlapping_windows(P):
+    """q rows that are windows of one vector, a column apart: empty_like lays such a tensor out with its columns not contiguous."""
+    from triton_ext_b200.rotary import Rope
+    q = torch.randn(200, device="cuda").bfloat16().unfold(0, 64, 1)[:10][None].transpose(0, 1)       # [10, 1, 64]
+    pages, table, kv = batch_of([1] * 10, [3] * 10, 16, 7)
+    pools = [torch.zeros(pages, 16, 1, 64, dtype=bf16, device="cuda") for _ in range(2)]
+    got = P.append(q, q, q, *pools, table, kv, rope=Rope(64))
+    want = P.append(q.clone(memory_format=torch.contiguous_format), q, q, *pools, table, kv, rope=Rope(64))
+    P.check()
+    assert torch.equal(got, want)
+
+
 def test_append_with_bad_pages_and_lengths(P):
     """Entries outside the cache, positions past the table and lengths below the new tokens write nothing and are reported."""
     from triton_ext_b200 import backend as B

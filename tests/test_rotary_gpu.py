@@ -149,6 +149,17 @@ def test_both_tensors_have_to_be_copied(R):
     assert torch.equal(gq, one) and torch.equal(gk, 2 * one)
 
 
+def test_overlapping_windows(R):
+    """Rows that are windows of one vector, a column apart: empty_like lays such a tensor out with its columns not contiguous."""
+    rope = R.Rope(64)
+    x = torch.randn(200, device="cuda").unfold(0, 64, 1)[:10]          # strides (1, 1)
+    for q in (x[None, None], x[:, None][None], x[None, None].bfloat16().as_strided((1, 1, 10, 64), (640, 640, 1, 1))):
+        pos = torch.arange(q.shape[2], device="cuda")
+        got, _ = R.rotary_forward(q, None, pos, rope)
+        want, _ = R.rotary_forward(q.clone(memory_format=torch.contiguous_format), None, pos, rope)
+        assert torch.equal(got, want) and got.is_contiguous()
+
+
 def test_empty(R):
     rope = R.Rope(32)
     q, k = tensor((2, 3, 0, 64), bf16, 1), tensor((2, 1, 0, 64), bf16, 1)

@@ -140,6 +140,9 @@ def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages:
         if out is None:
             out = torch.empty_like(q)
             os_ = out.stride()
+            if os_[2] != 1:  # q is made of overlapping windows: its layout is none to follow
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                os_ = out.stride()
         else:
             os_ = _token_strides(out, "out", tokens, d, k_pages, device)
             if out.shape != q.shape or (tokens > 1 and os_[0] == 0) or (q_heads > 1 and os_[1] == 0):

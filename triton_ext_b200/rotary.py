@@ -129,6 +129,8 @@ def _part(x: torch.Tensor, out: Optional[torch.Tensor], heads: int, name: str):
         a = x.stride()
     if out is None:
         out = torch.empty_like(x)
+        if out.stride(3) != 1:  # x is made of overlapping windows: its layout is none to follow
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
     b = out.stride()
     return _PART.pack(x.data_ptr(), out.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], heads, 0), out, x
 
