@@ -112,8 +112,8 @@ TXD_API int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_p
 /* The pages of a cache and who holds them. k and v: [layers, num_pages, page_bytes]; table: [rows, width], -1 where a row
  * has no page; lens[row]: its tokens; refs[page]: in how many table cells it stands (0: free). All on the device, changed
  * in stream order, without the host. What is wrong with a call is found on the device and reported by tx_paged_check: a
- * row outside the table is passed over by free and fork; a reserve with such a row, a row listed twice, a negative count,
- * no room in a row or too few free pages does nothing at all.
+ * row outside the table is passed over by free, truncate and fork; a reserve with such a row, a row listed twice, a negative
+ * count, no room in a row or too few free pages does nothing at all.
  * `workspace`: tx_pages_workspace(state, n) bytes, 16-byte aligned, of the caller; free again when the call has run. */
 typedef struct tx_pages_state {
   void *k, *v;
@@ -127,6 +127,10 @@ typedef struct tx_pages_state {
 TXD_API int64_t tx_pages_workspace(const tx_pages_state *state, int32_t n);
 /* Gives the pages of the listed rows back and empties the rows (a row may be listed twice). */
 TXD_API int tx_pages_free(const tx_pages_state *state, const int32_t *rows, int32_t n, void *stream);
+/* Cuts the listed rows to keep[i] tokens (drafted tokens that were not accepted) and gives the pages behind those back. A row
+ * that is no longer than that keeps its length; one listed twice ends at the lesser; a negative keep[i] is passed over.
+ * Lengths are shortened by this call, not in lens: a reserve takes the cells behind a row's length for empty. */
+TXD_API int tx_pages_truncate(const tx_pages_state *state, const int32_t *rows, const int32_t *keep, int32_t n, void *stream);
 /* Row dst[i] becomes what row src[i] was before the call, sharing its pages; what dst[i] held is given back. Sources may be
  * destinations too (a reordering); where a destination is listed twice the last one holds. */
 TXD_API int tx_pages_fork(const tx_pages_state *state, const int32_t *dst, const int32_t *src, int32_t n, void *workspace,

@@ -204,3 +204,15 @@ def test_cache_refuses():
                  (k[:, :, :, :, ::2], k[:, :, :, :, ::2], table, lens, refs)):
         with pytest.raises(B.DotError):
             P.PagedCache(*args)
+
+
+def test_truncate_refuses(built_libs):
+    lib = P._lib()
+    state = P._STATE.pack(1 << 20, 1 << 20, 64, 1 << 20, 1 << 20, 1 << 20, 1, 8, 16, 4, 4, 0)
+    assert lib.tx_pages_truncate(state, None, 1 << 20, 1, None) == B.TXD_ERR_INVALID
+    assert lib.tx_pages_truncate(state, 1 << 20, None, 1, None) == B.TXD_ERR_INVALID
+    assert lib.tx_pages_truncate(state, 1 << 20, 1 << 20, -1, None) == B.TXD_ERR_INVALID
+    assert lib.tx_pages_truncate(state, None, None, 0, None) == B.TXD_OK
+    cache = P.PagedCache.create(4, 16, 2, 64, rows=3, width=2, device="cpu")
+    rows = torch.zeros(1, dtype=i32)
+    assert status_of(lambda: cache.truncate(rows, rows))[0] == B.TXD_ERR_NO_DEVICE

@@ -467,3 +467,58 @@ def test_a_serving_run(P, page, d, dtype):
     assert bool((cache.refs[:used] > 0).all())
     step([0, 1, 2, 3, 4, 5], [1, 40, 1, 17, 1, 1])
     P.check()
+
+
+@pytest.mark.parametrize("page,window,captured", [(16, 0, False), (32, 40, True)])
+def test_drafts_that_are_not_accepted(P, page, window, captured):
+    """Five drafted tokens for each row, of which as many are kept as a device tensor says: the step is reserve, append,
+    attention, truncate, eager or captured once and replayed. No page is lost, and every step's attention is that over the
+    kept tokens and the drafts."""
+    from triton_ext_b200.rotary import Rope
+    g = torch.Generator().manual_seed(page)
+    rng = random.Random(page)
+    d, h, hk, rows, drafts = 64, 4, 2, 3, 5
+    cache = P.PagedCache.create(30, page, hk, d, rows=rows, width=128 // page, dtype=bf16)
+    every, count, kept = ints(range(rows)), ints([drafts] * rows), ints([drafts] * rows)
+    cu = ints(range(0, drafts * rows + 1, drafts))
+    q, k, v = (torch.zeros(drafts * rows, n, d, dtype=bf16, device="cuda") for n in (h, hk, hk))
+
+    def step():
+        cache.reserve(every, count)
+        P.append(None, k, v, cache.k[0], cache.v[0], cache.table, cache.lens, cu_q=cu)
+        out = P.paged_attention(q, cache.k[0], cache.v[0], cache.table, cache.lens, 0.125, cu_q=cu, max_q=drafts, window=window)
+        cache.truncate(every, cache.lens - drafts + kept)
+        return out
+
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+    keys, values = [[] for _ in range(rows)], [[] for _ in range(rows)]
+    for _ in range(12):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g).bfloat16())
+        keep = [rng.randint(0, drafts) for _ in range(rows)]
+        kept.copy_(ints(keep))
+        if captured:
+            graph.replay()
+        else:
+            out = step()
+        for r in range(rows):
+            new = slice(r * drafts, (r + 1) * drafts)
+            kk, vv = (torch.stack(a + list(b[new])).double().repeat_interleave(h // hk, 1).transpose(0, 1)
+                      for a, b in ((keys[r], k.clone()), (values[r], v.clone())))
+            s = q[new].double().transpose(0, 1) @ kk.transpose(1, 2) * 0.125
+            pos = torch.arange(len(keys[r]), len(keys[r]) + drafts, device="cuda")[:, None]
+            key = torch.arange(kk.shape[1], device="cuda")
+            hidden = (key > pos) | (key <= pos - window if window else key < 0)
+            want = (s.masked_fill(hidden, -math.inf).softmax(-1) @ vv).transpose(0, 1)
+            # u for the output and u for P, of at most the largest |v| (below 5); a third for all the rest (2^-11 and less)
+            assert float((out[new].double() - want).abs().max()) <= 3 * 5 * 2.0 ** -8
+            keys[r] += list(k[new].clone()[: keep[r]])
+            values[r] += list(v[new].clone()[: keep[r]])
+    P.check()
+    lens = [len(x) for x in keys]
+    assert cache.lens.tolist() == lens
+    assert [sum(p >= 0 for p in r) for r in cache.table.tolist()] == [-(-n // page) for n in lens]
+    assert int(cache.refs.sum()) == sum(-(-n // page) for n in lens)

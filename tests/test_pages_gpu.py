@@ -145,6 +145,43 @@ def test_shared_last_pages(P):
     P.check()
 
 
+def test_truncate(P):
+    """Whole and part pages, shared ones, to nothing, to more than there is, a row twice; then the rows grow again."""
+    from triton_ext_b200 import backend as B
+    cache, model = make(P)
+
+    def cut(rows, keep):
+        for r, n in zip(rows, keep):
+            while len(model.rows[r]) * model.page >= max(n, 0) + model.page:
+                model.refs[model.rows[r].pop()] -= 1
+            model.lens[r] = min(model.lens[r], n)
+        cache.truncate(ints(*rows), ints(*keep))
+
+    cache.reserve(ints(0, 1, 2), ints(100, 5, 64))
+    model.reserve([0, 1, 2], [100, 5, 64])
+    cache.fork(ints(3, 4, 5), ints(0, 0, 2))
+    model.fork([3, 4, 5], [0, 0, 2])
+    for rows, keep in (([0, 1], [97, 5]), ([2, 3], [49, 32]), ([4, 4, 4], [70, 33, 50]), ([5, 1, 0], [0, 9, 2 ** 31 - 1]), ([], [])):
+        cut(rows, keep)
+        model.same_as(cache)
+        P.check()
+    grow = [3, 2, 4, 0, 5, 1], [20, 1, 16, 1, 3, 40]                    # row 4 ends inside a page that row 0 holds
+    cache.reserve(ints(*grow[0]), ints(*grow[1]))
+    model.reserve(*grow)
+    model.same_as(cache)
+    for rows, keep, text in ((ints(10, -1, 0), ints(1, 1, 60), "outside the table"), (ints(1, 2), ints(-1, 50), "below zero")):
+        cache.truncate(rows, keep)
+        with pytest.raises(B.DotError, match=text):
+            P.check()
+    for r, n in ((0, 60), (2, 50)):
+        while len(model.rows[r]) * model.page >= n + model.page:
+            model.refs[model.rows[r].pop()] -= 1
+        model.lens[r] = n
+    model.same_as(cache)
+    with pytest.raises(B.DotError, match="keep must be an int32 vector of 2"):
+        cache.truncate(ints(1, 2), ints(1))
+
+
 def test_many_pages_and_rows(P):
     """More pages than one step of the planning block (16384) looks at, a list longer than the block, and a full cache."""
     cache, model = make(P, pages=40000, page=16, heads=1, d=16, rows=2000, width=20, layers=1)

@@ -328,6 +328,18 @@ int tx_pages_free(const tx_pages_state *st, const int32_t *rows, int32_t n, void
   return TXD_OK;
 }
 
+int tx_pages_truncate(const tx_pages_state *st, const int32_t *rows, const int32_t *keep, int32_t n, void *stream) {
+  int rc = check_pages(st);
+  if (rc) return rc;
+  if (n < 0 || (n > 0 && (!rows || !keep))) return fail(TXD_ERR_INVALID, "lists of n >= 0 rows and lengths are wanted");
+  if (n == 0) return TXD_OK;
+  PagesParams p = {};
+  if ((rc = pages_params(st, nullptr, &p))) return rc;
+  TXP_CUDA(launch(pages_truncate_kernel, dim3(n), dim3(256), 0, static_cast<cudaStream_t>(stream), p, rows, keep));
+  count_launches(1);
+  return TXD_OK;
+}
+
 int tx_pages_fork(const tx_pages_state *st, const int32_t *dst, const int32_t *src, int32_t n, void *workspace, void *stream) {
   int rc = check_pages(st);
   if (rc) return rc;

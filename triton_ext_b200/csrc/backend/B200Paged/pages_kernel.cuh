@@ -49,6 +49,28 @@ __global__ void __launch_bounds__(256) pages_free_kernel(const __grid_constant__
   if (threadIdx.x == 0) p.lens[row] = 0;
 }
 
+// Rows are cut to keep[i] tokens (drafts that were not accepted); a row listed twice ends at the lesser, whatever the order
+// of the blocks: the length is a minimum, and the exchange hands each page to one of the two only.
+__global__ void __launch_bounds__(256) pages_truncate_kernel(const __grid_constant__ PagesParams p, const int32_t *rows,
+                                                             const int32_t *keep) {
+  grid_dep_wait();
+  const int row = rows[blockIdx.x], tokens = keep[blockIdx.x];
+  if (row < 0 || row >= p.rows || tokens < 0) {
+    if (threadIdx.x == 0) atomicOr(p.status, row < 0 || row >= p.rows ? kBadRow : kBadLength);
+    return;
+  }
+  const long long first = (static_cast<long long>(tokens) + (1ll << p.page_shift) - 1) >> p.page_shift;
+  for (long long c = first + threadIdx.x; c < p.width; c += 256) {
+    int32_t *cell = p.table + row * static_cast<long long>(p.width) + c;
+    const int page = *cell < 0 ? -1 : atomicExch(cell, -1);
+    if (page >= 0) {
+      if (page < p.num_pages) atomicSub(&p.refs[page], 1);
+      else atomicOr(p.status, kBadPage);
+    }
+  }
+  if (threadIdx.x == 0) atomicMin(&p.lens[row], tokens);
+}
+
 // A fork runs as two kernels: the first takes the source rows as they are and counts the new holders, the second gives
 // up what the destinations held and writes them. Between them every source has been read, so rows may be both.
 __device__ __forceinline__ bool fork_listed_later(const int32_t *dst, int n, int i) {

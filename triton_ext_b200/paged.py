@@ -2,7 +2,7 @@
 
   append            the new tokens' k (turned by their positions) and v into their pages, and the turned q
   paged_attention   the new tokens' attention over their sequences' pages: chunks of a prompt, drafted tokens, single tokens
-  PagedCache        who holds which page, on the device: reserve, fork, free, compact, copy_pages
+  PagedCache        who holds which page, on the device: reserve, truncate, fork, free, compact, copy_pages
 
 A step is `cache.reserve(rows, counts)`, then for every layer `append` and `paged_attention`. Nothing in a step
 synchronises, reads the device or depends on the host knowing a length, so a step can be captured in a CUDA graph and
@@ -39,6 +39,7 @@ def _lib() -> ctypes.CDLL:
                 ("tx_paged_attention_workspace", [vp, vp], i64),
                 ("tx_pages_workspace", [vp, i32], i64),
                 ("tx_pages_free", [vp, vp, i32, vp], ctypes.c_int),
+                ("tx_pages_truncate", [vp, vp, vp, i32, vp], ctypes.c_int),
                 ("tx_pages_fork", [vp, vp, vp, i32, vp, vp], ctypes.c_int),
                 ("tx_pages_reserve", [vp, vp, vp, i32, vp, vp], ctypes.c_int),
                 ("tx_pages_compact", [vp, vp, vp], ctypes.c_int),
@@ -211,7 +212,7 @@ class PagedCache:
     k, v    [layers, pages, page_size, kv_heads, head_dim], contiguous, f16 or bf16; `k[layer]` is what `append` and
             `paged_attention` take
     table   int32 [rows, width]: the pages of each row (a sequence), -1 where there is none
-    lens    int32 [rows]: its tokens
+    lens    int32 [rows]: its tokens (to be read; the operations change it)
     refs    int32 [pages]: in how many table cells a page stands; 0: free
 
     The operations take rows as int32 CUDA vectors, run in stream order and never synchronise; a row outside the table is
@@ -259,6 +260,13 @@ class PagedCache:
         """Give the pages of the listed rows back (those that no other row holds become free) and empty the rows."""
         lib, rows = _lib(), self._list(rows, "rows")
         _call(rows.get_device(), lib.tx_pages_free, self._state, rows.data_ptr(), rows.shape[0])
+
+    def truncate(self, rows: torch.Tensor, keep: torch.Tensor) -> None:
+        """Cut row rows[i] to keep[i] tokens (drafted tokens that were not accepted) and give the pages behind them back; a row
+        that is no longer keeps its length. Rows are shortened by this, not by writing to `lens`."""
+        lib, rows = _lib(), self._list(rows, "rows")
+        keep = self._list(keep, "keep", rows.shape[0])
+        _call(rows.get_device(), lib.tx_pages_truncate, self._state, rows.data_ptr(), keep.data_ptr(), rows.shape[0])
 
     def fork(self, dst: torch.Tensor, src: torch.Tensor) -> None:
         """Row dst[i] becomes what row src[i] was before the call, sharing its pages. Rows may be both (the reordering of a
