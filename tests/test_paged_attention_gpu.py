@@ -405,6 +405,18 @@ def test_refusals(P):
     P.check()
 
 
+def test_bounds_past_32_bits(P):
+    """A window or a bound on the new tokens beyond every length is as good as none."""
+    from triton_ext_b200 import backend as B
+    b = Batch([3, 40], [30, 70], 4, 2, 64, 16, bf16)
+    want = b.run(P, 0.1)
+    assert torch.equal(b.run(P, 0.1, window=2 ** 40, max_q=2 ** 40), want)
+    assert torch.equal(b.run(P, 0.1, window=2 ** 31 - 1, max_q=2 ** 31 - 1), want)
+    for kw in (dict(window=-2 ** 40), dict(max_q=-2 ** 40)):
+        with pytest.raises(B.DotError):
+            b.run(P, 0.1, **kw)
+
+
 # ---- a run of the operators together ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("page,d,dtype", [(16, 64, bf16), (64, 128, f16)])
 def test_a_serving_run(P, page, d, dtype):

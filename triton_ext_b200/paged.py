@@ -24,6 +24,7 @@ from .rotary import Rope, _call, check  # noqa: F401  (check: part of this modul
 
 _DTYPES = {torch.float16: B.TXD_F16, torch.bfloat16: B.TXD_BF16}
 MAX_LIST = 4096  # rows in one reserve
+_INT_MAX = 2 ** 31 - 1
 
 _lib_cache = None
 
@@ -199,7 +200,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             _invalid("out must have the shape of q and not be an expanded tensor")
     m = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_m else None
     problem = _ATTN.pack(q.data_ptr(), out.data_ptr(), m.data_ptr() if return_m else 0, qs[0], qs[1], os_[0], os_[1], tokens,
-                         heads, max_q, 1 if causal else 0, window, sm_scale)
+                         heads, min(max(max_q, -1), _INT_MAX), 1 if causal else 0, min(max(window, -1), _INT_MAX), sm_scale)
     size = lib.tx_paged_attention_workspace(view, problem)
     ws = q.new_empty((size + 1) // 2)  # 16-bit values
     _call(device, lib.tx_paged_attention, view, problem, ws.data_ptr(), size)
