@@ -113,7 +113,7 @@ TXD_API int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_p
  * has no page; lens[row]: its tokens; refs[page]: in how many table cells it stands (0: free). All on the device, changed
  * in stream order, without the host. What is wrong with a call is found on the device and reported by tx_paged_check: a
  * row outside the table is passed over by free, truncate and fork; a reserve with such a row, a row listed twice, a negative
- * count, no room in a row or too few free pages does nothing at all.
+ * count, no room in a row or too few free pages does nothing at all (what that means for the step behind it: tx_pages_reserve_lens).
  * `workspace`: tx_pages_workspace(state, n) bytes, 16-byte aligned, of the caller; free again when the call has run. */
 typedef struct tx_pages_state {
   void *k, *v;
@@ -140,6 +140,13 @@ TXD_API int tx_pages_fork(const tx_pages_state *state, const int32_t *dst, const
  * the last keeps it). */
 TXD_API int tx_pages_reserve(const tx_pages_state *state, const int32_t *rows, const int32_t *counts, int32_t n,
                              void *workspace, void *stream);
+/* The same, and step_lens[i] (device, n values) becomes the new length of row rows[i], or TX_PAGES_REFUSED in all of them where
+ * the call did nothing. What follows without the host knowing which it was takes its lengths from there, not from lens:
+ * as kv_lens a refused length writes nothing to the cache and sees no key (rows of zeros), and as keep (step_lens - drafted +
+ * accepted) it cuts nothing. With lens a step behind a refused reserve would take the last old tokens for its new ones. */
+#define TX_PAGES_REFUSED (-(1 << 30)) /* below zero whatever numbers of tokens are added to it */
+TXD_API int tx_pages_reserve_lens(const tx_pages_state *state, const int32_t *rows, const int32_t *counts, int32_t n,
+                                  int32_t *step_lens, void *workspace, void *stream);
 /* Moves pages so that the used ones are the lowest: with U pages in use, those at U and above go to the free ones below, in
  * order, and the table follows. */
 TXD_API int tx_pages_compact(const tx_pages_state *state, void *workspace, void *stream);

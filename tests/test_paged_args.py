@@ -216,3 +216,15 @@ def test_truncate_refuses(built_libs):
     cache = P.PagedCache.create(4, 16, 2, 64, rows=3, width=2, device="cpu")
     rows = torch.zeros(1, dtype=i32)
     assert status_of(lambda: cache.truncate(rows, rows))[0] == B.TXD_ERR_NO_DEVICE
+
+
+def test_reserve_with_lengths_refuses(built_libs):
+    """The checks of a plain reserve, and nothing to do for an empty list."""
+    lib = P._lib()
+    state = P._STATE.pack(1 << 20, 1 << 20, 64, 1 << 20, 1 << 20, 1 << 20, 1, 8, 16, 4, 4, 0)
+    call = lib.tx_pages_reserve_lens
+    assert call(None, 1 << 20, 1 << 20, 1, 1 << 20, 1 << 20, None) == B.TXD_ERR_INVALID
+    assert call(state, None, 1 << 20, 1, 1 << 20, 1 << 20, None) == B.TXD_ERR_INVALID
+    assert call(state, 1 << 20, 1 << 20, P.MAX_LIST + 1, 1 << 20, 1 << 20, None) == B.TXD_ERR_UNSUPPORTED
+    assert call(state, 1 << 20, 1 << 20, 1, 1 << 20, None, None) == B.TXD_ERR_INVALID  # workspace
+    assert call(state, None, None, 0, None, None, None) == B.TXD_OK

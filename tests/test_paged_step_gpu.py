@@ -1,0 +1,134 @@
+"""Steps over a paged cache in which something goes wrong: what must not be touched, and what `check` has to report."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+bf16, i32 = torch.bfloat16, torch.int32
+
+
+@pytest.fixture(scope="module")
+def P(built_libs, cuda_device):
+    from triton_ext_b200 import paged
+    return paged
+
+
+def ints(*x):
+    return torch.tensor(x, dtype=i32, device="cuda")
+
+
+def everything(cache):
+    """The cache's state as whole numbers (pools hold NaN)."""
+    return [x.clone().view(torch.int16 if x.dtype == bf16 else i32) for x in (cache.k, cache.v, cache.table, cache.lens, cache.refs)]
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ---- a reserve that cannot be done ---------------------------------------------------------------------------------------
+DRAFTS = 3
+
+
+def short_of_pages(P, page=16):
+    """Rows 0 and 1 share their 20 tokens, row 2 holds every other page: no row can grow into a new page."""
+    cache = P.PagedCache.create(6, page, 2, 64, rows=4, width=6, layers=2)
+    cache.k.fill_(math.nan)
+    cache.v.fill_(math.nan)
+    lens = cache.reserve(ints(0), ints(20))
+    g = torch.Generator().manual_seed(40)
+    k, v = (torch.randn(20, 2, 64, generator=g).to(bf16).cuda() for _ in range(2))
+    for layer in range(2):
+        P.append(None, k, v, cache.k[layer], cache.v[layer], cache.table[:1], lens, cu_q=ints(0, 20))
+    cache.fork(ints(1), ints(0))
+    assert cache.reserve(ints(2), ints(64)).tolist() == [64]
+    P.check()
+    assert cache.refs.tolist() == [2, 2, 1, 1, 1, 1] and lens.tolist() == [20]
+    return cache
+
+
+def one_step(P, cache, rows, counts, kept, q, k, v, cu, causal=True):
+    lens = cache.reserve(rows, counts)
+    table, out = cache.table[rows.clamp(0, 3).long()], []
+    for layer in range(2):
+        P.append(None, k, v, cache.k[layer], cache.v[layer], table, lens, cu_q=cu)
+        out.append(P.paged_attention(q, cache.k[layer], cache.v[layer], table, lens, 0.125, cu_q=cu, max_q=DRAFTS, causal=causal, return_m=True))
+    cache.truncate(rows, lens - counts + kept)
+    return lens, out
+
+
+def step_tensors(tokens):
+    g = torch.Generator().manual_seed(41)
+    return [torch.randn(tokens, n, 64, generator=g).to(bf16).cuda() for n in (4, 2, 2)]
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_refused_reserve_stops_its_step(P, captured, causal):
+    """No free page for a copy of the shared last page: reserve, append, attention and truncate leave pools, table, lengths and
+    counts as they were, the sibling's tokens among them. With room made the same step goes through."""
+    from triton_ext_b200 import backend as B
+    cache = short_of_pages(P)
+    rows, counts, kept, cu = ints(0), ints(DRAFTS), ints(1), ints(0, DRAFTS)
+    q, k, v = step_tensors(DRAFTS)
+    before = everything(cache)
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            lens, out = one_step(P, cache, rows, counts, kept, q, k, v, cu, causal)
+    for _ in range(2):
+        if captured:
+            graph.replay()
+        else:
+            lens, out = one_step(P, cache, rows, counts, kept, q, k, v, cu, causal)
+        with pytest.raises(B.DotError, match="no free pages"):
+            P.check()
+        assert lens.tolist() == [-(1 << 30)]
+        assert same(everything(cache), before)
+        for o, m in out:
+            assert bool((o == 0).all()) and bool((m == -math.inf).all())
+    cache.free(ints(2))
+    if captured:
+        graph.replay()
+    else:
+        lens, out = one_step(P, cache, rows, counts, kept, q, k, v, cu, causal)
+    P.check()
+    assert lens.tolist() == [20 + DRAFTS] and cache.lens.tolist() == [21, 20, 0, 0]
+    copied = int(cache.table[0, 1])
+    assert cache.table[1, :2].tolist() == [0, 1] and copied == 2 and cache.refs.tolist() == [2, 1, 1, 0, 0, 0]
+    for pool, old, new in ((cache.k, before[0], k), (cache.v, before[1], v)):
+        assert torch.equal(pool.view(torch.int16)[:, :2], old[:, :2])                       # what row 1 sees
+        assert torch.equal(pool.view(torch.int16)[:, copied, :4], old[:, 1, :4])
+        assert torch.equal(pool[:, copied, 4:4 + DRAFTS], new[None].expand(2, -1, -1, -1))
+    assert all(bool((o != 0).any()) and bool(m.isfinite().all()) for o, m in out)
+
+
+@pytest.mark.parametrize("rows,counts,text", [((0, 3), (3, 90), "no free pages"), ((3, 0), (3, 96), "width"), ((0, 0), (3, 3), "listed twice"),
+                                             ((3, 9), (3, 3), "outside the table"), ((3, 1), (3, -3), "negative count")])
+def test_one_row_that_has_no_room_stops_the_batch(P, rows, counts, text):
+    """Whatever row of a batch cannot be served, none of its rows are touched by the step."""
+    from triton_ext_b200 import backend as B
+    cache = short_of_pages(P)
+    cache.free(ints(2))
+    before = everything(cache)
+    q, k, v = step_tensors(2 * DRAFTS)
+    lens, out = one_step(P, cache, ints(*rows), ints(*counts), ints(1, 1), q, k, v, ints(0, DRAFTS, 2 * DRAFTS))
+    with pytest.raises(B.DotError, match=text):
+        P.check()
+    assert lens.tolist() == [-(1 << 30)] * 2 and same(everything(cache), before)
+    assert all(bool((o == 0).all()) for o, m in out)
+
+
+def test_the_lengths_of_a_step(P):
+    """Row by row of the list, rows that do not grow and an empty list among them; more rows than the planning block has threads."""
+    cache = P.PagedCache.create(4000, 16, 1, 16, rows=3000, width=4)
+    g = torch.Generator().manual_seed(42)
+    rows = torch.randperm(3000, generator=g).to(i32).cuda()
+    first, more = (torch.randint(0, 7, (3000,), generator=g).to(i32).cuda() for _ in range(2))
+    assert torch.equal(cache.reserve(rows, first), first)
+    assert torch.equal(cache.reserve(rows[:1500], more[:1500]), (first + more)[:1500])
+    assert torch.equal(cache.lens[rows.long()][1500:], first[1500:])
+    assert cache.reserve(rows[:0], more[:0]).shape == (0,)
+    P.check()

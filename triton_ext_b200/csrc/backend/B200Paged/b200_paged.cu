@@ -357,6 +357,11 @@ int tx_pages_fork(const tx_pages_state *st, const int32_t *dst, const int32_t *s
 
 int tx_pages_reserve(const tx_pages_state *st, const int32_t *rows, const int32_t *counts, int32_t n, void *workspace,
                      void *stream) {
+  return tx_pages_reserve_lens(st, rows, counts, n, nullptr, workspace, stream);
+}
+
+int tx_pages_reserve_lens(const tx_pages_state *st, const int32_t *rows, const int32_t *counts, int32_t n, int32_t *step_lens,
+                          void *workspace, void *stream) {
   int rc = check_pages(st);
   if (rc) return rc;
   if (n < 0 || (n > 0 && (!rows || !counts))) return fail(TXD_ERR_INVALID, "lists of n >= 0 rows and counts are wanted");
@@ -369,7 +374,7 @@ int tx_pages_reserve(const tx_pages_state *st, const int32_t *rows, const int32_
   if ((rc = set_plan_smem())) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const size_t smem = (4 * static_cast<size_t>(n) + (st->rows + 31) / 32) * 4;
-  TXP_CUDA(launch(pages_reserve_plan_kernel, dim3(1), dim3(kPlanThreads), smem, s, p, rows, counts, n));
+  TXP_CUDA(launch(pages_reserve_plan_kernel, dim3(1), dim3(kPlanThreads), smem, s, p, rows, counts, n, step_lens));
   TXP_CUDA(launch(pages_copy_kernel, dim3(copy_grid(st, n)), dim3(256), 0, s, p));
   count_launches(2);
   return TXD_OK;

@@ -157,13 +157,19 @@ __device__ __forceinline__ void load_refs(const PagesParams &p, int first, int (
   }
 }
 
+// A reserve is done for all of its rows or for none. step_lens (may be NULL) carries that to the kernels behind it, which are
+// launched without the host knowing: the rows' new lengths, or kRefused. Without it an append behind a reserve that found no
+// free pages would take the last old tokens' places, in pages that other rows may hold as well.
+constexpr int32_t kRefused = TX_PAGES_REFUSED;
+
 // Dynamic shared memory: end[n], last[n] (last page of the row if it is partly filled, else -1), row[n], len[n],
 // seen[rows / 32]. What takes the time is loads that wait for one another, so each is made once and the first step's
 // reference counts are loaded before anything else.
 constexpr int kFreshShared = 2048;  // free pages that are handed on in shared memory
 
 __global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan_kernel(const __grid_constant__ PagesParams p,
-                                                                          const int32_t *rows, const int32_t *counts, int n) {
+                                                                          const int32_t *rows, const int32_t *counts, int n,
+                                                                          int32_t *step_lens) {
   extern __shared__ int32_t plan_smem[];
   __shared__ int warp_sums[32], s_fresh[kFreshShared];
   __shared__ int s_bad, s_pairs;
@@ -257,6 +263,8 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan_kernel(const 
       atomicOr(p.status, static_cast<uint32_t>(s_bad) | (found < need_all ? kNoFreePages : 0u));
       p.ws[0] = 0;
     }
+    if (step_lens)
+      for (int i = tid; i < n; i += kPlanThreads) step_lens[i] = kRefused;
     return;
   }
   for (int r = tid; r < need_all; r += kPlanThreads) {
@@ -278,7 +286,11 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan_kernel(const 
       atomicSub(&p.refs[last[lo]], 1);
     }
   }
-  for (int i = tid; i < n; i += kPlanThreads) p.lens[s_row[i]] = s_len[i] + counts[i];
+  for (int i = tid; i < n; i += kPlanThreads) {
+    const int len = s_len[i] + counts[i];
+    p.lens[s_row[i]] = len;
+    if (step_lens) step_lens[i] = len;
+  }
   __syncthreads();
   if (tid == 0) p.ws[0] = s_pairs;
 }

@@ -4,9 +4,10 @@
   paged_attention   the new tokens' attention over their sequences' pages: chunks of a prompt, drafted tokens, single tokens
   PagedCache        who holds which page, on the device: reserve, truncate, fork, free, compact, copy_pages
 
-A step is `cache.reserve(rows, counts)`, then for every layer `append` and `paged_attention`. Nothing in a step
-synchronises, reads the device or depends on the host knowing a length, so a step can be captured in a CUDA graph and
-replayed while the sequences grow. What kernels find wrong (a bad page, no free pages) is reported by `check`.
+A step is `lens = cache.reserve(rows, counts)`, then for every layer `append` and `paged_attention` with those lengths. Nothing
+in a step synchronises, reads the device or depends on the host knowing a length, so a step can be captured in a CUDA graph
+and replayed while the sequences grow. What kernels find wrong (a bad page, no free pages) is reported by `check`; a step whose
+`reserve` was refused leaves the cache as it was.
 
 torch is used for device memory and streams only. There is no fallback: if the shared library is missing or no B200 is
 present the calls raise.
@@ -43,6 +44,7 @@ def _lib() -> ctypes.CDLL:
                 ("tx_pages_truncate", [vp, vp, vp, i32, vp], ctypes.c_int),
                 ("tx_pages_fork", [vp, vp, vp, i32, vp, vp], ctypes.c_int),
                 ("tx_pages_reserve", [vp, vp, vp, i32, vp, vp], ctypes.c_int),
+                ("tx_pages_reserve_lens", [vp, vp, vp, i32, vp, vp, vp], ctypes.c_int),
                 ("tx_pages_compact", [vp, vp, vp], ctypes.c_int),
                 ("tx_pages_copy", [vp, vp, vp, i32, vp], ctypes.c_int)):
             f = getattr(lib, name)
@@ -213,7 +215,7 @@ class PagedCache:
     k, v    [layers, pages, page_size, kv_heads, head_dim], contiguous, f16 or bf16; `k[layer]` is what `append` and
             `paged_attention` take
     table   int32 [rows, width]: the pages of each row (a sequence), -1 where there is none
-    lens    int32 [rows]: its tokens (to be read; the operations change it)
+    lens    int32 [rows]: its tokens (to be read; the operations change it). A step takes its lengths from `reserve` instead
     refs    int32 [pages]: in how many table cells a page stands; 0: free
 
     The operations take rows as int32 CUDA vectors, run in stream order and never synchronise; a row outside the table is
@@ -277,14 +279,22 @@ class PagedCache:
         ws = self._workspace(lib, dst)
         _call(dst.get_device(), lib.tx_pages_fork, self._state, dst.data_ptr(), src.data_ptr(), dst.shape[0], ws.data_ptr())
 
-    def reserve(self, rows: torch.Tensor, counts: torch.Tensor) -> None:
+    def reserve(self, rows: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
         """Make room for counts[i] more tokens in row rows[i] and add them to its length, before they are appended. New pages
         are the lowest free ones in list order. A partly filled last page that other rows share is copied first (all layers);
-        of the listed rows that alone share one, the last keeps it."""
+        of the listed rows that alone share one, the last keeps it.
+
+        Returns the rows' new lengths, int32 [n], for the step that follows: `kv_lens` of `append` and `paged_attention`, and
+        less the drafts that were not accepted, `keep` of `truncate`. Where there is no room nothing is done for any row, and
+        they are far below zero: append then writes nothing to the cache, attention gives zeros, truncate cuts nothing, and
+        `check` reports it. (`lens` stays as it was: an append with it would overwrite the rows' last tokens.)"""
         lib, rows = _lib(), self._list(rows, "rows")
         counts = self._list(counts, "counts", rows.shape[0])
         ws = self._workspace(lib, rows)
-        _call(rows.get_device(), lib.tx_pages_reserve, self._state, rows.data_ptr(), counts.data_ptr(), rows.shape[0], ws.data_ptr())
+        lens = rows.new_empty(rows.shape[0])
+        _call(rows.get_device(), lib.tx_pages_reserve_lens, self._state, rows.data_ptr(), counts.data_ptr(), rows.shape[0],
+              lens.data_ptr(), ws.data_ptr())
+        return lens
 
     def compact(self) -> None:
         """Move pages (all layers) so that the used ones are the lowest, the fewest that do it; the table follows."""
