@@ -132,3 +132,26 @@ def test_the_lengths_of_a_step(P):
     assert torch.equal(cache.lens[rows.long()][1500:], first[1500:])
     assert cache.reserve(rows[:0], more[:0]).shape == (0,)
     P.check()
+
+
+# ---- what check reports ------------------------------------------------------------------------------------------------
+def small_cache():
+    g = torch.Generator().manual_seed(43)
+    return [torch.randn(8, 16, 2, 64, generator=g).to(bf16).cuda() for _ in range(2)]
+
+
+@pytest.mark.parametrize("q", [1, 100])
+def test_a_wait_that_runs_out_is_reported_with_what_was_found_before(P, q, monkeypatch):
+    """A page outside the cache is pending when the attention's wait runs out: both are in the report, as a time-out."""
+    from triton_ext_b200 import backend as B
+    pools = small_cache()
+    x = torch.ones(1, 2, 64, dtype=bf16, device="cuda")
+    P.append(None, x, x, *pools, ints(-1)[None], ints(1))
+    monkeypatch.setenv("TXD_INJECT_STALL", "1")
+    monkeypatch.setenv("TXD_WAIT_LIMIT_MS", "50")
+    qs = torch.ones(q, 4, 64, dtype=bf16, device="cuda")
+    P.paged_attention(qs, *pools, ints(0, 1, 2, 3, 4, 5, 6)[None], ints(112), 0.125, cu_q=ints(0, q), max_q=q)
+    with pytest.raises(B.DotError, match="ran out.*outside the cache") as e:
+        P.check()
+    assert e.value.status == B.TXD_ERR_DEVICE_TIMEOUT
+    P.check()

@@ -340,6 +340,10 @@ struct AbortCtl {
 // that starts the clock. The time limit therefore counts from the end of the polling phase.
 constexpr uint32_t kPollsBeforeTimer = 4096;
 
+// Part of a wait's code where the status word collects bits: the code is added to what stands there. Without it the word is
+// a single code, and the first one stays.
+constexpr uint32_t kStatusIsBits = 1u << 31;
+
 static __device__ __noinline__ bool mbar_wait_timed(uint32_t bar, uint32_t parity, const AbortCtl &ac,
                                              uint32_t code) {
   const unsigned long long t0 = global_timer_ns();
@@ -350,7 +354,8 @@ static __device__ __noinline__ bool mbar_wait_timed(uint32_t bar, uint32_t parit
       if (*ac.flag) return false;
       if (global_timer_ns() - t0 > ac.limit_ns) {
         *ac.flag = 1;
-        atomicCAS(ac.status, 0u, code);
+        if (code & kStatusIsBits) atomicOr(ac.status, code & ~kStatusIsBits);
+        else atomicCAS(ac.status, 0u, code);
         return false;
       }
     }

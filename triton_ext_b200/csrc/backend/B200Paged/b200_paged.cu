@@ -436,8 +436,9 @@ int tx_paged_check(void *stream) {
   TXP_CUDA(cudaMemcpy(&found, status, sizeof found, cudaMemcpyDeviceToHost));
   if (!found) return TXD_OK;
   TXP_CUDA(cudaMemset(status, 0, sizeof found));
-  if (found & kTimeout) return fail(TXD_ERR_DEVICE_TIMEOUT, "a bounded wait inside the paged attention kernel ran out");
-  return fail(TXD_ERR_INVALID, "on the device:%s%s%s%s%s", found & kBadPage ? " a page-table entry outside the cache;" : "",
+  return fail(found & kTimeout ? TXD_ERR_DEVICE_TIMEOUT : TXD_ERR_INVALID, "on the device:%s%s%s%s%s%s",
+              found & kTimeout ? " a bounded wait inside the paged attention kernel ran out;" : "",
+              found & kBadPage ? " a page-table entry outside the cache;" : "",
               found & kBadRow ? " a row outside the table, listed twice or with a negative count;" : "",
               found & kNoRoomInRow ? " a position past the width of the page table;" : "",
               found & kNoFreePages ? " no free pages;" : "",

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
     const uint32_t box_bytes = (128u << p.box_shift) * kGroups;
     auto hand_on = [&](bool more) {
       const uint32_t i = count % kRowItems;
-      if (!warp_mbar_poll(smem_u32(&item_empty[i]), ((count / kRowItems) & 1u) ^ 1u, ac, kTimeout, lane)) {
+      if (!warp_mbar_poll(smem_u32(&item_empty[i]), ((count / kRowItems) & 1u) ^ 1u, ac, kWaitRanOut, lane)) {
         ok = false;
         return;
       }
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
         const int id = __shfl_sync(0xffffffffu, page_reg, page & 31);
         const bool wanted = lane < 2 * boxes && tok < w.t.hi && tok + (1 << p.box_shift) > w.t.lo;
         const uint32_t count = __popc(__ballot_sync(0xffffffffu, wanted));
-        if (!warp_mbar_poll(smem_u32(&empty[slot]), (pass & 1u) ^ 1u, ac, kTimeout, lane)) {
+        if (!warp_mbar_poll(smem_u32(&empty[slot]), (pass & 1u) ^ 1u, ac, kWaitRanOut, lane)) {
           ok = false;
           break;
         }
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
       }
       if (ok && w.to > w.from) {  // the slot that the tile's warps are joined in
         const uint32_t slot = issued % kStages, pass = issued / kStages;
-        if (!warp_mbar_poll(smem_u32(&empty[slot]), (pass & 1u) ^ 1u, ac, kTimeout, lane)) ok = false;
+        if (!warp_mbar_poll(smem_u32(&empty[slot]), (pass & 1u) ^ 1u, ac, kWaitRanOut, lane)) ok = false;
         else if (lane == 0) mbar_arrive(smem_u32(&full[slot]));
         __syncwarp();
         ++issued;
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
     bool ok = true;
     auto take = [&]() -> uint32_t {
       const uint32_t slot = taken % kStages;
-      if (ok && !warp_mbar_poll(smem_u32(&full[slot]), (taken / kStages) & 1u, ac, kTimeout, lane)) ok = false;
+      if (ok && !warp_mbar_poll(smem_u32(&full[slot]), (taken / kStages) & 1u, ac, kWaitRanOut, lane)) ok = false;
       ++taken;
       return slot;
     };
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
 
     for (uint32_t count = 0;; ++count) {
       const uint32_t item = count % kRowItems;
-      if (ok && !warp_mbar_poll(smem_u32(&item_full[item]), (count / kRowItems) & 1u, ac, kTimeout, lane)) ok = false;
+      if (ok && !warp_mbar_poll(smem_u32(&item_full[item]), (count / kRowItems) & 1u, ac, kWaitRanOut, lane)) ok = false;
       if (any_of<kConsumers * 32>(!ok)) break;  // all of them leave, or none
       const RowItem w = items[item];
       __syncwarp();

@@ -23,6 +23,8 @@ namespace txp {
 
 using namespace txd;
 
+constexpr uint32_t kWaitRanOut = kTimeout | kStatusIsBits;  // what the kernels' bounded waits report
+
 struct Sched {
   const int32_t *kv_lens, *cu_q;
   int32_t batch, tokens, kv_heads, group;

@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   uint32_t item_count = 0;
   auto next_item = [&]() -> bool {
     const uint32_t i = item_count % kItems;
-    if (!warp_mbar_poll(smem_u32(&ctl.item_full[i]), (item_count / kItems) & 1u, ac, kTimeout, lane)) return false;
+    if (!warp_mbar_poll(smem_u32(&ctl.item_full[i]), (item_count / kItems) & 1u, ac, kWaitRanOut, lane)) return false;
     w = ctl.item[i];
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[i]));
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     for (bool more = walk.start(p.s, &sched), last = false; !last; more = more && walk.next(p.s, &sched), ++count) {
       last = !more;
       const uint32_t i = count % kItems;
-      if (!warp_mbar_wait(smem_u32(&ctl.item_empty[i]), ((count / kItems) & 1u) ^ 1u, ac, kTimeout, lane)) break;
+      if (!warp_mbar_wait(smem_u32(&ctl.item_empty[i]), ((count / kItems) & 1u) ^ 1u, ac, kWaitRanOut, lane)) break;
       if (lane == 0) {
         TileItem x = {};
         if (more) {
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     while (ok && next_item()) {
       const int nb = w.blocks;
       if (nb <= 0) continue;
-      if (!warp_mbar_poll(smem_u32(&ctl.q_empty), (items & 1u) ^ 1u, ac, kTimeout, lane)) {
+      if (!warp_mbar_poll(smem_u32(&ctl.q_empty), (items & 1u) ^ 1u, ac, kWaitRanOut, lane)) {
         ok = false;
         break;
       }
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const uint32_t bytes = (b1 - b0) * kAtoms * box_bytes;
         const int in_mask = (1 << p.page_shift) - 1;
         int id = __shfl_sync(0xffffffffu, ids, ((tok0 + (b0 << p.box_shift)) >> p.page_shift) & 31);
-        if (!warp_mbar_poll(smem_u32(&ctl.kv_empty[slot]), ((issued / kStages) & 1u) ^ 1u, ac, kTimeout, lane)) {
+        if (!warp_mbar_poll(smem_u32(&ctl.kv_empty[slot]), ((issued / kStages) & 1u) ^ 1u, ac, kWaitRanOut, lane)) {
           ok = false;
           return;
         }
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     bool ok = true;
     auto take = [&]() -> uint32_t {
       const uint32_t slot = taken % kStages;
-      if (!warp_mbar_poll(smem_u32(&ctl.kv_full[slot]), (taken / kStages) & 1u, ac, kTimeout, lane)) ok = false;
+      if (!warp_mbar_poll(smem_u32(&ctl.kv_full[slot]), (taken / kStages) & 1u, ac, kWaitRanOut, lane)) ok = false;
       ++taken;
       return slot;
     };
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       // S of block j: after the accumulator's last S has been read into registers (one tile's last before the next one's first)
       auto next_s = [&](int t, int j, uint32_t k_slot) {
         if (j >= n_blk[t]) return;
-        if (s_count[t] > 0 && !warp_mbar_poll(smem_u32(&ctl.s_free[t]), (s_count[t] - 1) & 1u, ac, kTimeout, lane)) {
+        if (s_count[t] > 0 && !warp_mbar_poll(smem_u32(&ctl.s_free[t]), (s_count[t] - 1) & 1u, ac, kWaitRanOut, lane)) {
           ok = false;
           return;
         }
@@ -384,14 +384,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       };
       auto update_o = [&](int t, int j, uint32_t v_slot) {
         if (j >= n_blk[t]) return;
-        if (!warp_mbar_poll(smem_u32(&ctl.p_full[t]), p_count[t] & 1u, ac, kTimeout, lane)) {
+        if (!warp_mbar_poll(smem_u32(&ctl.p_full[t]), p_count[t] & 1u, ac, kWaitRanOut, lane)) {
           ok = false;
           return;
         }
         tc_fence_after();
         issue_pv(t, v_slot, j > 0);
       };
-      if (!warp_mbar_poll(smem_u32(&ctl.q_full), items & 1u, ac, kTimeout, lane)) {
+      if (!warp_mbar_poll(smem_u32(&ctl.q_full), items & 1u, ac, kWaitRanOut, lane)) {
         ok = false;
         break;
       }
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       const int seen_lo = ((p.s.window ? max(w.pos0 + w.tokens - p.s.window, 0) : 0) + 127 >> 7) - w.block;
       float m_i = -INFINITY, l_i = 0.f;
       for (int j = 0; j < n; ++j, ++count) {
-        if (!warp_mbar_poll(smem_u32(&ctl.s_full[t]), count & 1u, ac, kTimeout, lane)) {
+        if (!warp_mbar_poll(smem_u32(&ctl.s_full[t]), count & 1u, ac, kWaitRanOut, lane)) {
           ok = false;
           break;
         }
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const float alpha = fast_exp2(m_i - ref);
         if (count > 0) {
           // the last O update of this sub-tile has completed: P may be overwritten and O rescaled
-          if (!warp_mbar_poll(smem_u32(&ctl.o_done[t]), (count - 1) & 1u, ac, kTimeout, lane)) {
+          if (!warp_mbar_poll(smem_u32(&ctl.o_done[t]), (count - 1) & 1u, ac, kWaitRanOut, lane)) {
             ok = false;
             break;
           }
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       if (!ok) break;
       // ---- the tile's end ----
       if (n > 0) {
-        ok = warp_mbar_poll(smem_u32(&ctl.o_done[t]), (count - 1) & 1u, ac, kTimeout, lane);
+        ok = warp_mbar_poll(smem_u32(&ctl.o_done[t]), (count - 1) & 1u, ac, kWaitRanOut, lane);
         if (!ok) break;
         tc_fence_after();
       }
