@@ -153,7 +153,9 @@ TXD_API int tx_pages_compact(const tx_pages_state *state, void *workspace, void 
 /* Copies pages src[i] to dst[i] in every layer (host lists). No page may be a destination twice, or source and destination. */
 TXD_API int tx_pages_copy(const tx_pages_state *state, const int32_t *src, const int32_t *dst, int32_t n, void *stream);
 
-/* Synchronises `stream` and reports (and clears) what kernels of this header found on the device since the last check. */
+/* Synchronises `stream` and reports (and clears, in one step) what kernels of this header found on the device since the last
+ * check. The word is the device's: a check also reports, and so takes from other threads' checks, what kernels on other
+ * streams have found by then; what they find later stays for the next check. */
 TXD_API int tx_paged_check(void *stream);
 
 TXD_API uint64_t tx_paged_kernel_launches(void);

@@ -155,3 +155,66 @@ def test_a_wait_that_runs_out_is_reported_with_what_was_found_before(P, q, monke
         P.check()
     assert e.value.status == B.TXD_ERR_DEVICE_TIMEOUT
     P.check()
+
+
+def test_no_finding_of_another_stream_is_lost(P):
+    """A kernel on a side stream reports a bad page while the main stream checks over and over, each time with a finding of its
+    own to clear: one of the checks has the page in its report, whenever the kernel ran."""
+    from triton_ext_b200 import backend as B
+    pools = small_cache()
+    x, side = torch.ones(1, 2, 64, dtype=bf16, device="cuda"), torch.cuda.Stream()
+    bad, good, one, short = ints(-1)[None], ints(0)[None], ints(1), ints(-3)
+    torch.cuda.synchronize()
+
+    def found():
+        with pytest.raises(B.DotError) as e:
+            P.append(None, x, x, *pools, good, short)
+            P.check()
+        return "outside the cache" in str(e.value)
+
+    lost = 0
+    for i in range(150):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200000 + 7919 * i % 200000)
+            P.append(None, x, x, *pools, bad, one)
+            done = torch.cuda.Event()
+            done.record()
+        times = 0
+        while not done.query():
+            times += found()
+        times += found()
+        assert times <= 1                                         # and none is reported twice
+        lost += times == 0
+    assert lost == 0, f"{lost} of 150 findings lost"
+    P.check()
+
+
+def test_checks_of_two_threads_at_once(P):
+    """Each finding is in exactly one report, whichever thread's."""
+    import threading
+
+    from triton_ext_b200 import backend as B
+    pools, x, streams = small_cache(), torch.ones(1, 2, 64, dtype=bf16, device="cuda"), [torch.cuda.Stream() for _ in range(2)]
+    bad, one, reports, wrong = ints(-1)[None], ints(1), [0, 0], []
+    torch.cuda.synchronize()
+
+    def run(i):
+        try:
+            with torch.cuda.stream(streams[i]):
+                for _ in range(200):
+                    if i == 0:
+                        P.append(None, x, x, *pools, bad, one)
+                    try:
+                        P.check()
+                    except B.DotError as e:
+                        reports[i] += "outside the cache" in str(e)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and sum(reports) == 200
+    P.check()

@@ -224,7 +224,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
 
 def check(device=None) -> None:
     """Synchronise the current stream and raise for what the rotary, append, paged attention and page kernels found wrong
-    on the device since the last check."""
+    on the device since the last check, on this stream and, as far as they have run, on others. Nothing goes unreported, but
+    where several threads check one device, any of them may be the one that is told."""
     index = None if device is None else device if isinstance(device, int) else torch.device(device).index
     lib = _lib()
     _call(torch.cuda.current_device() if index is None else index, lib.tx_paged_check)
