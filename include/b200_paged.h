@@ -61,9 +61,11 @@ TXD_API int tx_rotary(const tx_rope *rope, const tx_rotary_problem *problem, con
  * slot p % page_size. k and v: [num_pages, page_size, kv_heads, head_dim] with head_dim contiguous and the other strides
  * free (multiples of 16 bytes). `kv_lens[b]` counts the cached tokens with the new ones; `cu_q` [batch + 1] holds where
  * each sequence's new tokens start among all new tokens (NULL: one new token for each sequence). Sequence b's new tokens
- * are its last ones: token j of q_len has position kv_lens[b] - q_len + j. Table entries that no used position needs are
- * not read; an entry outside [0, num_pages) that is needed reads as zeros, is not written, and is reported by
- * tx_paged_check. */
+ * are its last ones: token j of q_len has position kv_lens[b] - q_len + j. cu_q starts at or above zero, never falls and ends at
+ * or below the number of new tokens. Where it does not, or a length is negative or beyond the table's row, tx_paged_check
+ * reports it: a token with no place in the table is not written, a negative length sees no keys, and beyond that what the
+ * call gives for the sequences concerned has no meaning. Table entries that no used position needs are not read; an entry
+ * outside [0, num_pages) that is needed reads as zeros, is not written, and is reported by tx_paged_check. */
 typedef struct tx_paged_view {
   void *k, *v;
   int64_t k_stride[3], v_stride[3]; /* page, slot, head; in elements */
@@ -90,7 +92,8 @@ TXD_API int tx_paged_append(const tx_paged_view *cache, const tx_rope *rope, con
 /* Attention of the new tokens over their sequences' cached keys and values (which include their own: append first).
  * Query head h reads key head h / (q_heads / kv_heads). With `causal` new token j sees the keys at positions up to its own,
  * kv_lens[b] - q_len + j, and with `window` > 0 only the last `window` of them; without `causal` it sees all kv_lens[b].
- * A row that sees no key gives zeros and m = -inf. What the cache holds at positions that no row of a sequence sees never
+ * A row that sees no key gives zeros and m = -inf (so do the first tokens where kv_lens[b] < q_len: attention allows that, an
+ * append reports it). What the cache holds at positions that no row of a sequence sees never
  * matters (it may be NaN); keys and values that some row sees have to be finite.
  * `m` (may be NULL): [tokens, q_heads] fp32, running max + log2(sum) in base 2 as tx_attn_fwd returns it. Rows behind the
  * last sequence are left alone. `max_q` is the caller's bound on the new tokens of one sequence: it decides between the

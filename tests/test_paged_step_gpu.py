@@ -218,3 +218,41 @@ def test_checks_of_two_threads_at_once(P):
         t.join()
     assert not wrong and sum(reports) == 200
     P.check()
+
+
+@pytest.mark.parametrize("tokens", [6, 300])
+@pytest.mark.parametrize("what,cu,lens,text", [
+    ("length", (0, 3, 6), (10, -1), "below zero"), ("length", None, (-5, 10), "below zero"),
+    ("falling", (0, 4, 2), (10, 10), "cu_q that fall"), ("below", (-2, 3, 6), (10, 10), "outside the new tokens"),
+    ("behind", (0, 3, 9), (10, 20), "outside the new tokens")])
+def test_lengths_and_offsets_that_cannot_be_are_reported(P, tokens, what, cu, lens, text):
+    """By append and by attention (both of its kernels), which stay inside their tensors."""
+    from triton_ext_b200 import backend as B
+    pools, table = small_cache(), torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=i32, device="cuda")
+    rows = 2 if cu is None else tokens
+    if cu is not None:
+        cu, lens = ints(*(c * tokens // 6 for c in cu)), tuple(n if n < 0 else min(48, n * tokens // 6) for n in lens)
+    q, out = (torch.full((rows + 2, 4, 64), x, dtype=bf16, device="cuda") for x in (1.0, 9.0))
+    kw = dict(cu_q=cu, max_q=tokens) if cu is not None else {}
+    P.paged_attention(q[:rows], *pools, table, ints(*lens), 0.125, out=out[:rows], **kw)
+    with pytest.raises(B.DotError, match=text):
+        P.check()
+    assert bool((out[rows:] == 9.0).all()) and not bool(out.isnan().any())
+    before = [x.clone() for x in pools]
+    k = torch.ones(rows, 2, 64, dtype=bf16, device="cuda")
+    P.append(None, k, k, *pools, table, ints(*lens), cu_q=cu)
+    with pytest.raises(B.DotError, match=text):
+        P.check()
+    assert all(torch.equal(a[6:], b[6:]) for a, b in zip(pools, before))        # pages that are nobody's
+
+
+def test_more_new_tokens_than_cached_ones_are_no_fault(P):
+    """For attention: the first rows see nothing. And offsets that leave rows before, between none and behind are as they should be."""
+    pools, table = small_cache(), torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=i32, device="cuda")
+    q = torch.ones(40, 4, 64, dtype=bf16, device="cuda")
+    for cu, lens in (((3, 20, 33), (5, 20)), ((0, 0, 40), (0, 40)), ((0, 0, 0), (0, 0)), ((40, 40, 40), (7, 7))):
+        P.paged_attention(q, *pools, table, ints(*lens), 0.125, cu_q=ints(*cu), max_q=40)
+        P.check()
+        if lens[0] >= cu[1] - cu[0] and lens[1] >= cu[2] - cu[1]:
+            P.append(None, q[:, :2], q[:, :2], *pools, table, ints(*lens), cu_q=ints(*cu))
+            P.check()

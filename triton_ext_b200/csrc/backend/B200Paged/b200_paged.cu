@@ -451,13 +451,14 @@ int tx_paged_check(void *stream_v) {
     TXP_CUDA(cudaStreamSynchronize(s));
   }
   if (!found) return TXD_OK;
-  return fail(found & kTimeout ? TXD_ERR_DEVICE_TIMEOUT : TXD_ERR_INVALID, "on the device:%s%s%s%s%s%s",
+  return fail(found & kTimeout ? TXD_ERR_DEVICE_TIMEOUT : TXD_ERR_INVALID, "on the device:%s%s%s%s%s%s%s",
               found & kTimeout ? " a bounded wait inside the paged attention kernel ran out;" : "",
               found & kBadPage ? " a page-table entry outside the cache;" : "",
               found & kBadRow ? " a row outside the table, listed twice or with a negative count;" : "",
               found & kNoRoomInRow ? " a position past the width of the page table;" : "",
               found & kNoFreePages ? " no free pages;" : "",
-              found & kBadLength ? " a length below zero or below the number of new tokens;" : "");
+              found & kBadLength ? " a length below zero or below the number of new tokens;" : "",
+              found & kBadOffsets ? " offsets in cu_q that fall or lie outside the new tokens;" : "");
 }
 
 }  // extern "C"

@@ -16,8 +16,9 @@ enum PagedStatus : uint32_t {
   kBadRow = 2u,       // a row index outside the table, a row listed twice, or a negative count
   kNoRoomInRow = 4u,  // a position past the width of the page table
   kNoFreePages = 8u,
-  kBadLength = 16u,   // more new tokens than cached tokens
-  kTimeout = 32u      // a bounded wait ran out
+  kBadLength = 16u,   // a negative length, or in an append more new tokens than cached tokens
+  kTimeout = 32u,     // a bounded wait ran out
+  kBadOffsets = 64u   // offsets of new tokens that fall or lie outside the tokens
 };
 
 int fail(int code, const char *fmt, ...);

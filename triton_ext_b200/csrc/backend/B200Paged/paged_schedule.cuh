@@ -200,7 +200,13 @@ __device__ __forceinline__ void find_work(const Sched &s, SchedSmem *sm, int4 *b
   SeqInfo q = {0, 0, 0};
   for (int b = tid; b < s.batch; b += kThreads) {
     q = seq_info(s, b);
-    if (cta == 0 && s.kv_lens[b] > s.max_kv) atomicOr(s.status, kNoRoomInRow);
+    if (cta == 0) {
+      // what seq_info has cut to size (fewer cached tokens than new ones are allowed: the first ones see nothing)
+      const int len = s.kv_lens[b];
+      uint32_t bad = len > s.max_kv ? kNoRoomInRow : len < 0 ? kBadLength : 0u;
+      if (s.cu_q && (s.cu_q[b] < 0 || s.cu_q[b + 1] < s.cu_q[b] || s.cu_q[b + 1] > s.tokens)) bad |= kBadOffsets;
+      if (bad) atomicOr(s.status, bad);
+    }
     per_head = head_cost(s, q);
     mine += per_head * s.kv_heads;
   }

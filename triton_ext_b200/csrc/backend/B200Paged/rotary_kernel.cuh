@@ -153,11 +153,18 @@ __global__ void __launch_bounds__(kRotaryThreads, 8) rotary_kernel(const __grid_
   // ---- the token's position, and where an append puts it ----
   long long pos, page = -1, z = 0, n = t;
   if (append) {
+    if (id == 0 && p.cu_q) {  // one warp looks at all offsets
+      bool bad = p.cu_q[0] < 0 || p.cu_q[p.batch] > static_cast<int>(p.total);
+      for (int b = lane; b < p.batch; b += 32) bad |= p.cu_q[b + 1] < p.cu_q[b];
+      if (bad) atomicOr(p.status, kBadOffsets);
+    }
     const int s = p.cu_q ? find_sequence(p.cu_q, p.batch, static_cast<int>(t), lane) : static_cast<int>(t);
     if (s >= p.batch || (p.cu_q && p.cu_q[0] > static_cast<int>(t))) return;  // behind the last sequence
     pos = p.cu_q ? static_cast<long long>(p.kv_lens[s]) - (p.cu_q[s + 1] - static_cast<int>(t)) : p.kv_lens[s] - 1;
     uint32_t bad = 0;
-    if (pos < 0) {
+    if (p.cu_q && (p.cu_q[s + 1] <= static_cast<int>(t) || p.cu_q[s + 1] > static_cast<int>(p.total))) {
+      bad = kBadOffsets;  // which sequence the token belongs to, or where in it, is not known
+    } else if (pos < 0) {
       bad = kBadLength;
     } else if ((pos >> p.page_shift) >= p.table_width) {
       bad = kNoRoomInRow;
