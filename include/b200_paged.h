@@ -117,7 +117,8 @@ TXD_API int tx_paged_attention(const tx_paged_view *cache, const tx_paged_attn_p
  * in stream order, without the host. What is wrong with a call is found on the device and reported by tx_paged_check: a
  * row outside the table is passed over by free, truncate and fork; a reserve with such a row, a row listed twice, a negative
  * count, no room in a row or too few free pages does nothing at all (what that means for the step behind it: tx_pages_reserve_lens).
- * `workspace`: tx_pages_workspace(state, n) bytes, 16-byte aligned, of the caller; free again when the call has run. */
+ * `workspace`: tx_pages_workspace(state, n) bytes, 16-byte aligned, of the caller; free again when the call has run. Lists of rows,
+ * counts and lengths are not parts of the state's arrays, which change while they are read. */
 typedef struct tx_pages_state {
   void *k, *v;
   int64_t page_bytes; /* of one layer's k (or v), a multiple of 16 */

@@ -256,3 +256,37 @@ def test_more_new_tokens_than_cached_ones_are_no_fault(P):
         if lens[0] >= cu[1] - cu[0] and lens[1] >= cu[2] - cu[1]:
             P.append(None, q[:, :2], q[:, :2], *pools, table, ints(*lens), cu_q=ints(*cu))
             P.check()
+
+
+# ---- lists that are parts of the cache's own state -------------------------------------------------------------------------
+def test_lists_out_of_the_caches_lengths(P):
+    """Rows cut to other rows' lengths, and grown by them: the lengths as they are before the call. More blocks and rows than run
+    at once, in an order in which every length changes before it is read where the lists are not copied first."""
+    n = 2000
+    cache = P.PagedCache.create(3 * n, 16, 1, 16, rows=3 * n, width=4)
+    every = torch.arange(3 * n, dtype=i32, device="cuda")
+    sixteen = torch.full((n,), 16, dtype=i32, device="cuda")
+    cache.reserve(every[n:2 * n], sixteen)
+    cache.reserve(every[2 * n:], sixteen)
+    cache.truncate(every[n:], cache.lens[:2 * n])                  # the second third to the first's 0, the last to the second's 16
+    assert cache.lens.tolist() == [0] * (2 * n) + [16] * n and int(cache.refs.sum()) == n
+    P.check()
+    cache = P.PagedCache.create(3 * n, 16, 1, 16, rows=n, width=40)
+    first = torch.arange(n, dtype=i32, device="cuda") % 7 + 1
+    cache.reserve(every[:n], first)
+    want = first + first.flip(0)
+    lens = cache.reserve(every[:n].flip(0), cache.lens)
+    assert torch.equal(cache.lens, want) and torch.equal(lens, want.flip(0))
+    P.check()
+
+
+def test_lists_out_of_the_caches_table(P):
+    """Any of the state's arrays may be a list."""
+    cache = P.PagedCache.create(8, 16, 1, 16, rows=4, width=3)
+    assert cache.reserve(ints(0, 1, 3), ints(40, 20, 5)).tolist() == [40, 20, 5]   # pages 0 1 2, 3 4, 5
+    cache.fork(cache.table[0], cache.table[1, :1].expand(3))        # rows 0, 1, 2 become row 3
+    P.check()
+    assert cache.lens.tolist() == [5, 5, 5, 5] and cache.table[:, 0].tolist() == [5] * 4 and cache.refs.tolist() == [0] * 5 + [4, 0, 0]
+    cache.free(cache.refs[:2])                                      # row 0, twice
+    P.check()
+    assert cache.lens.tolist() == [0, 5, 5, 5] and cache.refs.tolist() == [0] * 5 + [3, 0, 0]

@@ -237,6 +237,9 @@ class PagedCache:
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
         layers, pages, page_size, heads, d = k.shape
         self.page_size = page_size
+        self._workspaces = {}  # their sizes, by the length of a list
+        self._device = k.get_device()  # below zero: not a CUDA device
+        self._own = tuple(x for t in (table, lens, refs) for x in (t.data_ptr(), t.data_ptr() + 4 * t.numel()))
         self._state = _STATE.pack(k.data_ptr(), v.data_ptr(), page_size * heads * d * k.element_size(), table.data_ptr(),
                                   lens.data_ptr(), refs.data_ptr(), layers, pages, page_size, table.shape[0], table.shape[1], 0)
 
@@ -250,34 +253,43 @@ class PagedCache:
                    torch.zeros(pages, dtype=torch.int32, device=k.device))
 
     def _list(self, x: torch.Tensor, name: str, n: Optional[int] = None) -> torch.Tensor:
-        if not self.k.is_cuda:
+        if self._device < 0:
             _not_cuda(self.k)
-        if x.dtype != torch.int32 or x.dim() != 1 or x.device != self.k.device or (n is not None and x.shape[0] != n):
+        shape = x.shape
+        if x.dtype != torch.int32 or len(shape) != 1 or x.get_device() != self._device or (n is not None and shape[0] != n):
             _invalid(f"{name} must be an int32 vector{f' of {n}' if n is not None else ''} on the device of the cache")
-        return x if x.is_contiguous() else x.contiguous()
+        # a part of the state (lengths as counts, say) would change under the kernel that reads it
+        at, (t0, t1, l0, l1, r0, r1) = x.data_ptr(), self._own
+        if not x.is_contiguous() or l0 <= at < l1 or t0 <= at < t1 or r0 <= at < r1:
+            return x.clone(memory_format=torch.contiguous_format)
+        return x
 
-    def _workspace(self, lib, rows: torch.Tensor) -> torch.Tensor:
-        return rows.new_empty((lib.tx_pages_workspace(self._state, rows.shape[0]) + 3) // 4)
+    def _workspace(self, lib, n: int) -> torch.Tensor:
+        ints = self._workspaces.get(n)
+        if ints is None:
+            ints = self._workspaces[n] = (lib.tx_pages_workspace(self._state, n) + 3) // 4
+        return self.refs.new_empty(ints)
 
     def free(self, rows: torch.Tensor) -> None:
         """Give the pages of the listed rows back (those that no other row holds become free) and empty the rows."""
-        lib, rows = _lib(), self._list(rows, "rows")
-        _call(rows.get_device(), lib.tx_pages_free, self._state, rows.data_ptr(), rows.shape[0])
+        lib, rows = _lib_cache or _lib(), self._list(rows, "rows")
+        _call(self._device, lib.tx_pages_free, self._state, rows.data_ptr(), rows.shape[0])
 
     def truncate(self, rows: torch.Tensor, keep: torch.Tensor) -> None:
         """Cut row rows[i] to keep[i] tokens (drafted tokens that were not accepted) and give the pages behind them back; a row
         that is no longer keeps its length. Rows are shortened by this, not by writing to `lens`."""
-        lib, rows = _lib(), self._list(rows, "rows")
+        lib, rows = _lib_cache or _lib(), self._list(rows, "rows")
         keep = self._list(keep, "keep", rows.shape[0])
-        _call(rows.get_device(), lib.tx_pages_truncate, self._state, rows.data_ptr(), keep.data_ptr(), rows.shape[0])
+        _call(self._device, lib.tx_pages_truncate, self._state, rows.data_ptr(), keep.data_ptr(), rows.shape[0])
 
     def fork(self, dst: torch.Tensor, src: torch.Tensor) -> None:
         """Row dst[i] becomes what row src[i] was before the call, sharing its pages. Rows may be both (the reordering of a
         beam search); what a destination held is given back; of a destination listed twice the last one holds."""
-        lib, dst = _lib(), self._list(dst, "dst")
-        src = self._list(src, "src", dst.shape[0])
-        ws = self._workspace(lib, dst)
-        _call(dst.get_device(), lib.tx_pages_fork, self._state, dst.data_ptr(), src.data_ptr(), dst.shape[0], ws.data_ptr())
+        lib, dst = _lib_cache or _lib(), self._list(dst, "dst")
+        n = dst.shape[0]
+        src = self._list(src, "src", n)
+        ws = self._workspace(lib, n)
+        _call(self._device, lib.tx_pages_fork, self._state, dst.data_ptr(), src.data_ptr(), n, ws.data_ptr())
 
     def reserve(self, rows: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
         """Make room for counts[i] more tokens in row rows[i] and add them to its length, before they are appended. New pages
@@ -288,27 +300,27 @@ class PagedCache:
         less the drafts that were not accepted, `keep` of `truncate`. Where there is no room nothing is done for any row, and
         they are far below zero: append then writes nothing to the cache, attention gives zeros, truncate cuts nothing, and
         `check` reports it. (`lens` stays as it was: an append with it would overwrite the rows' last tokens.)"""
-        lib, rows = _lib(), self._list(rows, "rows")
-        counts = self._list(counts, "counts", rows.shape[0])
-        ws = self._workspace(lib, rows)
-        lens = rows.new_empty(rows.shape[0])
-        _call(rows.get_device(), lib.tx_pages_reserve_lens, self._state, rows.data_ptr(), counts.data_ptr(), rows.shape[0],
-              lens.data_ptr(), ws.data_ptr())
+        lib, rows = _lib_cache or _lib(), self._list(rows, "rows")
+        n = rows.shape[0]
+        counts = self._list(counts, "counts", n)
+        ws, lens = self._workspace(lib, n), rows.new_empty(n)
+        _call(self._device, lib.tx_pages_reserve_lens, self._state, rows.data_ptr(), counts.data_ptr(), n, lens.data_ptr(),
+              ws.data_ptr())
         return lens
 
     def compact(self) -> None:
         """Move pages (all layers) so that the used ones are the lowest, the fewest that do it; the table follows."""
-        lib = _lib()
-        if not self.k.is_cuda:
+        lib = _lib_cache or _lib()
+        if self._device < 0:
             _not_cuda(self.k)
-        ws = self.refs.new_empty((lib.tx_pages_workspace(self._state, 0) + 3) // 4)
-        _call(self.k.get_device(), lib.tx_pages_compact, self._state, ws.data_ptr())
+        ws = self._workspace(lib, 0)
+        _call(self._device, lib.tx_pages_compact, self._state, ws.data_ptr())
 
     def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
         """Copy the contents of pages src[i] to dst[i] in every layer. Host lists; no page may be a destination twice, or
         source and destination."""
         lib, n = _lib(), len(src)
-        if not self.k.is_cuda:
+        if self._device < 0:
             _not_cuda(self.k)
         if len(dst) != n:
             _invalid("src and dst must be of one length")
@@ -316,4 +328,4 @@ class PagedCache:
         for x in (*src, *dst):
             if not 0 <= int(x) < pages:
                 _invalid(f"page {x} is outside the {pages} pages")
-        _call(self.k.get_device(), lib.tx_pages_copy, self._state, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n)
+        _call(self._device, lib.tx_pages_copy, self._state, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n)
