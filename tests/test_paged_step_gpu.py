@@ -290,3 +290,53 @@ def test_lists_out_of_the_caches_table(P):
     cache.free(cache.refs[:2])                                      # row 0, twice
     P.check()
     assert cache.lens.tolist() == [0, 5, 5, 5] and cache.refs.tolist() == [0] * 5 + [3, 0, 0]
+
+
+# ---- inputs that require a gradient ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_backward_through_the_serving_operators_raises(P, in_place):
+    """Neither operator has a gradient: whoever asks for one is told, instead of getting the other paths' alone."""
+    from triton_ext_b200 import backend as B
+    from triton_ext_b200.rotary import Rope
+    pools, table, lens = small_cache(), ints(0, 1, 2)[None], ints(40)
+    leaf = torch.randn(1, 4, 64, device="cuda").to(bf16).requires_grad_()
+    k = torch.ones(1, 2, 64, dtype=bf16, device="cuda")
+
+    def loss(step):
+        return step(leaf * 2).float().sum() + (leaf * 3).float().sum()
+
+    def attend(x):
+        out, m = P.paged_attention(x, *pools, table, lens, 0.125, out=x if in_place else None, return_m=True)
+        assert out.requires_grad and m.requires_grad
+        return out
+
+    def turn(x):
+        return P.append(x, k, k, *pools, table, lens, rope=Rope(64), out=x if in_place else None)
+
+    def keys(x):
+        return P.append(leaf.detach(), x[:, :2], x[:, 2:], *pools, table, lens, rope=Rope(64))
+
+    for step, name in ((attend, "paged_attention"), (turn, "append"), (keys, "append")):
+        value = loss(step)
+        with pytest.raises(B.DotError, match=f"{name} has no gradient"):
+            value.backward()
+        assert leaf.grad is None or bool((leaf.grad == 3).all())
+        leaf.grad = None
+    P.check()
+
+
+def test_results_with_and_without_a_wanted_gradient_are_the_same(P):
+    pools, table, lens = small_cache(), ints(0, 1, 2)[None], ints(40)
+    q = torch.randn(1, 4, 64, device="cuda").to(bf16)
+    want = P.paged_attention(q, *pools, table, lens, 0.125, return_m=True)
+    got = P.paged_attention(q.clone().requires_grad_(), *pools, table, lens, 0.125, return_m=True)
+    assert torch.equal(got[0].detach(), want[0]) and torch.equal(got[1].detach(), want[1])
+    with torch.no_grad():
+        got = P.paged_attention(q.clone().requires_grad_(), *pools, table, lens, 0.125)
+    assert not got.requires_grad and torch.equal(got, want[0])
+    x = q.clone().requires_grad_() * 1
+    square = x * x                                                 # keeps x
+    assert P.paged_attention(x, *pools, table, lens, 0.125, out=x).data_ptr() == x.data_ptr()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        square.sum().backward()
+    P.check()

@@ -115,6 +115,25 @@ def _not_cuda(q: torch.Tensor):
     raise B.DotError(B.TXD_ERR_NO_DEVICE, f"CUDA tensors are wanted, got {q.device}: there is no CPU path")
 
 
+class _Forward(torch.autograd.Function):
+    """The result of an operator that has no gradient, for inputs that want one: a backward that reaches it raises."""
+
+    @staticmethod
+    def forward(ctx, name, out, m, *inputs):
+        ctx.name = name
+        return out, m
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise B.DotError(B.TXD_ERR_UNSUPPORTED, f"{ctx.name} has no gradient: it is for serving (use it under torch.no_grad)")
+
+
+def _without_gradient(name: str, out: torch.Tensor, m: Optional[torch.Tensor], *inputs: torch.Tensor):
+    if out.requires_grad:  # an input that was written in place: what a backward has kept of it is gone
+        torch.autograd.graph.increment_version(out)
+    return _Forward.apply(name, out, m, *inputs)
+
+
 def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
            page_table: torch.Tensor, kv_lens: torch.Tensor, *, rope: Optional[Rope] = None, cu_q: Optional[torch.Tensor] = None,
            out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
@@ -125,7 +144,8 @@ def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages:
     be None. k_pages, v_pages: [pages, page_size, kv_heads, head_dim]. page_table: int32 [batch, width]. kv_lens: int32
     [batch], the sequences' lengths WITH the new tokens. cu_q: int32 [batch + 1], where each sequence's new tokens start
     (None: one token for each sequence, in order). Sequence b's new tokens take its last positions. out: where the turned q
-    goes (q itself is allowed). Tokens behind cu_q[-1] are left alone: their rows of `out` are not written."""
+    goes (q itself is allowed). Tokens behind cu_q[-1] are left alone: their rows of `out` are not written.
+    There is no gradient: a backward through the result raises, and the cache carries none."""
     lib = _lib_cache or _lib()
     device = k.get_device()
     if device < 0:
@@ -159,6 +179,8 @@ def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages:
     problem = _APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1],
                            tokens, q_heads)
     _call(device, lib.tx_paged_append, view, rope._packed if rope is not None else None, problem)
+    if q is not None and (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        out, _ = _without_gradient("append", out, None, q, k, v)
     return out
 
 
@@ -173,7 +195,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     token sees the keys up to its own position (all keys of its sequence if not `causal`), with `window` > 0 the last `window`
     of them. max_q: a bound on the new tokens of one sequence, needed with cu_q. A row that sees nothing gives zeros.
     Returns the output, with `return_m` also [tokens, heads] fp32 of max + log2(sum) (base 2), -inf where nothing is seen.
-    Rows behind cu_q[-1] are left alone."""
+    Rows behind cu_q[-1] are left alone. There is no gradient: a backward through the result raises."""
     lib = _lib_cache or _lib()
     device = q.get_device()
     if device < 0:
@@ -206,6 +228,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     size = lib.tx_paged_attention_workspace(view, problem)
     ws = q.new_empty((size + 1) // 2)  # 16-bit values
     _call(device, lib.tx_paged_attention, view, problem, ws.data_ptr(), size)
+    if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
+        out, m = _without_gradient("paged_attention", out, m, q, k_pages, v_pages)
     return (out, m) if return_m else out
 
 
