@@ -1,5 +1,6 @@
 """Argument checks of the rotary and paged-cache binding that fire before any launch (no GPU), and the numbers behind a
 `Rope`."""
+import itertools
 import math
 import struct
 from fractions import Fraction
@@ -228,3 +229,24 @@ def test_reserve_with_lengths_refuses(built_libs):
     assert call(state, 1 << 20, 1 << 20, P.MAX_LIST + 1, 1 << 20, 1 << 20, None) == B.TXD_ERR_UNSUPPORTED
     assert call(state, 1 << 20, 1 << 20, 1, 1 << 20, None, None) == B.TXD_ERR_INVALID  # workspace
     assert call(state, None, None, 0, None, None, None) == B.TXD_OK
+
+
+@pytest.mark.parametrize("shape,strides,want", [
+    ((4, 3, 8), (24, 8, 1), False), ((4, 3, 8), (8, 32, 1), False), ((4, 3, 8), (100, 10, 1), False), ((1, 3, 8), (0, 8, 1), False),
+    ((4, 1, 8), (8, 0, 1), False), ((4, 3, 8), (0, 8, 1), True), ((4, 3, 8), (24, 0, 1), True), ((4, 3, 8), (8, 8, 1), True),
+    ((4, 1, 8), (1, 8, 1), True), ((4, 1, 8), (7, 8, 1), True), ((2, 4, 3, 8), (23, 8, 8, 1), True), ((1, 1, 1), (0, 0, 1), False),
+    ((0, 3, 8), (24, 8, 1), False)])
+def test_overlaps(shape, strides, want):
+    x = torch.zeros(500).as_strided(shape, strides)
+    assert R._overlaps(x) == want
+    if x.numel():
+        places = {sum(i * s for i, s in zip(at, strides)) for at in itertools.product(*(range(n) for n in shape))}
+        assert (len(places) < x.numel()) == want
+
+
+def test_outputs_that_overlap_themselves_are_refused():
+    """Windows of one vector, a column apart: rows would overwrite one another. Refused before there is a device to ask for."""
+    x = torch.zeros(2, 3, 10, 64)
+    with pytest.raises(B.DotError, match="overlap itself"):
+        R._part(x, torch.zeros(700).as_strided(x.shape, (300, 100, 1, 1)), 3, "out_q")
+    R._part(x, torch.zeros(2, 10, 3, 64).transpose(1, 2), 3, "out_q")

@@ -340,3 +340,17 @@ def test_results_with_and_without_a_wanted_gradient_are_the_same(P):
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         square.sum().backward()
     P.check()
+
+
+def test_outputs_that_overlap_themselves_are_refused(P):
+    from triton_ext_b200 import backend as B
+    pools, table = small_cache(), torch.zeros(10, 3, dtype=i32, device="cuda")
+    lens, x = torch.ones(10, dtype=i32, device="cuda"), torch.zeros(10, 2, 64, dtype=bf16, device="cuda")
+    memory = torch.full((4000,), 7.0, dtype=bf16, device="cuda")
+    for strides in ((1, 64, 1), (64, 64, 1), (8, 128, 1)):
+        out = memory.as_strided(x.shape, strides)
+        for call in (lambda: P.paged_attention(x, *pools, table, lens, 0.125, out=out), lambda: P.append(x, x, x, *pools, table, lens, out=out)):
+            with pytest.raises(B.DotError, match="overlap itself"):
+                call()
+    assert bool((memory == 7.0).all())
+    P.check()

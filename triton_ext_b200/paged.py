@@ -21,7 +21,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import backend as B
-from .rotary import Rope, _call, check  # noqa: F401  (check: part of this module's interface)
+from .rotary import Rope, _call, _overlaps, check  # noqa: F401  (check: part of this module's interface)
 
 _DTYPES = {torch.float16: B.TXD_F16, torch.bfloat16: B.TXD_BF16}
 MAX_LIST = 4096  # rows in one reserve
@@ -169,8 +169,8 @@ def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages:
                 os_ = out.stride()
         else:
             os_ = _token_strides(out, "out", tokens, d, k_pages, device)
-            if out.shape != q.shape or (tokens > 1 and os_[0] == 0) or (q_heads > 1 and os_[1] == 0):
-                _invalid("out must have the shape of q and not be an expanded tensor")
+            if out.shape != q.shape or _overlaps(out):
+                _invalid("out must have the shape of q and not be an expanded tensor, nor overlap itself in another way")
         q_ptr, o_ptr = q.data_ptr(), out.data_ptr()
     elif out is not None:
         _invalid("out is for the turned q: there is none")
@@ -220,8 +220,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         os_ = out.stride()
     else:
         os_ = _token_strides(out, "out", tokens, d, k_pages, device)
-        if out.shape != shape or (tokens > 1 and os_[0] == 0) or (heads > 1 and os_[1] == 0):
-            _invalid("out must have the shape of q and not be an expanded tensor")
+        if out.shape != shape or _overlaps(out):
+            _invalid("out must have the shape of q and not be an expanded tensor, nor overlap itself in another way")
     m = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_m else None
     problem = _ATTN.pack(q.data_ptr(), out.data_ptr(), m.data_ptr() if return_m else 0, qs[0], qs[1], os_[0], os_[1], tokens,
                          heads, min(max(max_q, -1), _INT_MAX), 1 if causal else 0, min(max(window, -1), _INT_MAX), sm_scale)

@@ -111,11 +111,21 @@ _PART = struct.Struct("2P6q2i")
 _NO_PART = _PART.pack(0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
+def _overlaps(x: torch.Tensor) -> bool:
+    """Whether elements of x may share their memory (expanded tensors, overlapping windows): no result can stand there."""
+    end = 0
+    for s, n in sorted((s, n) for n, s in zip(x.shape, x.stride()) if n > 1):
+        if s <= end:
+            return True
+        end += s * (n - 1)
+    return False
+
+
 def _check_out(out: torch.Tensor, x: torch.Tensor, name: str) -> None:
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
         raise B.DotError(B.TXD_ERR_INVALID, f"{name} must have its input's shape, type and device, HEAD_DIM contiguous")
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
-        raise B.DotError(B.TXD_ERR_INVALID, f"{name} must not be an expanded tensor")
+    if _overlaps(out):
+        raise B.DotError(B.TXD_ERR_INVALID, f"{name} must not be an expanded tensor, nor overlap itself in another way")
 
 
 def _part(x: torch.Tensor, out: Optional[torch.Tensor], heads: int, name: str):
@@ -141,7 +151,8 @@ def rotary_forward(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.
 
     q, k: [Z, H, N_CTX, HEAD_DIM] of one 16-bit type or float32 and any strides with HEAD_DIM contiguous (others are
     copied); k may have its own number of heads. positions: int32 or int64, [N_CTX] or [Z, N_CTX]. out_q, out_k: where the
-    results go (the inputs themselves are allowed: in place). inverse: turn backwards."""
+    results go (the inputs themselves are allowed: in place). inverse: turn backwards. No gradient is recorded: `rotary` is the
+    differentiable form."""
     lib = _lib_cache or _lib()
     shape = q.shape
     device = q.get_device()
