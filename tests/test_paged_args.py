@@ -250,3 +250,30 @@ def test_outputs_that_overlap_themselves_are_refused():
     with pytest.raises(B.DotError, match="overlap itself"):
         R._part(x, torch.zeros(700).as_strided(x.shape, (300, 100, 1, 1)), 3, "out_q")
     R._part(x, torch.zeros(2, 10, 3, 64).transpose(1, 2), 3, "out_q")
+
+
+@pytest.mark.parametrize("head_dim,tokens,rows,per_sm", [(16, 1, 16, 2), (64, 8, 16, 2), (128, 8, 16, 2), (64, 9, 32, 1), (128, 16, 32, 1),
+                                                         (32, 17, 256, 1), (64, 400, 256, 1), (128, 17, 256, 1), (256, 8, 16, 1),
+                                                         (256, 16, 32, 1), (256, 17, 64, 1), (256, 400, 64, 1)])
+def test_workspace_holds_the_parts_of_every_kernel(built_libs, head_dim, tokens, rows, per_sm):
+    """Two parts of a tile for each CTA: rows of fp32 columns, a maximum and a sum; and 16 bytes of border. Two query heads to a key
+    head; `rows` is the tile of the kernel that takes `tokens` of one sequence."""
+    lib = P._lib()
+    a = 1 << 20
+    view = P._VIEW.pack(a, a, 16 * 2 * head_dim, 2 * head_dim, head_dim, 16 * 2 * head_dim, 2 * head_dim, head_dim, a, 600, a, a, 1, 600,
+                        700, 16, 2, head_dim, B.TXD_BF16, 0)
+
+    def size(max_q):
+        return lib.tx_paged_attention_workspace(view, P._ATTN.pack(a, a, 0, 4 * head_dim, head_dim, 4 * head_dim, head_dim, tokens, 4, max_q,
+                                                                   1, 0, 0.1))
+
+    ctas = (torch.cuda.get_device_properties(0).multi_processor_count if torch.cuda.is_available() else 148) * per_sm
+    least = ctas * 2 * rows * (max(head_dim, 64) * 4 + 8) + 16 * ctas
+    assert least <= size(tokens) < least + 256
+    assert size(2 ** 31 - 1) == size(tokens)                       # the bound is cut to the tokens that there are
+    refused = lib.tx_paged_attention(view, P._ATTN.pack(a, a, 0, 4 * head_dim, head_dim, 4 * head_dim, head_dim, tokens, 4, tokens, 1, 0, 0.1),
+                                     a, size(tokens) - 1, None)
+    if torch.cuda.is_available():
+        assert refused == B.TXD_ERR_INVALID and f"of {size(tokens)} bytes" in lib.tx_paged_last_error().decode()
+    else:
+        assert refused == B.TXD_ERR_NO_DEVICE
