@@ -126,7 +126,8 @@ int make_plan(const tx_paged_view *cache, const tx_paged_attn_problem *pr, Plan 
   plan->rows = plan->tiled ? 256 : plan->shape.rows;
   plan->ctas = sm_count() * (plan->tiled ? 1 : plan->shape.per_sm);
   // Single tokens over at most 8 blocks: a tile is over sooner than a second kernel has joined its parts (1 sequence of 512
-  // tokens, 16 + 4 heads of 64: 10.2 us cut or whole, and a launch less; of 256 tokens: 7.9 us whole).
+  // tokens, 16 + 4 heads of 64: 10.2 us cut or whole, and a launch less; of 256 tokens: 7.9 us whole). The host knows what
+  // the table has room for and no length, so short sequences under a wide table are cut.
   plan->cuts = plan->tiled || static_cast<long long>(c.table_width) * c.page_size > 8 * plan->shape.block;
   plan->borders_bytes = (static_cast<size_t>(plan->ctas) * 16 + 255) / 256 * 256;
   const size_t rows = static_cast<size_t>(plan->ctas) * 2 * plan->rows;

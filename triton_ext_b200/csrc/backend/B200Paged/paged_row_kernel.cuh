@@ -370,7 +370,7 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
           mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
           mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)) * p.qk_scale;
           // the reference moves only when a score passes it by 2^8 (values stay below 2^8 times the exact ones: nothing is
-          // lost in fp32, and P rounds relative to itself)
+          // lost in fp32)
           grow |= mx[e] > m[e] + 8.f;
         }
         if (__any_sync(0xffffffffu, grow)) {
@@ -389,6 +389,9 @@ __global__ void __launch_bounds__((MT * KS + 1) * 32, kBlocksPerSm) paged_row_ke
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) ref[e] = m[e] == -INFINITY ? 0.f : -m[e];
+        // P is rounded to the cache's type for its product, as in the dense forward: the tensor instructions take 16-bit
+        // values, and a second product for what is rounded off would double the work. The sum takes the unrounded values.
+        // Outputs are off by 1.25 to 1.45 times what their own rounding costs (bf16: 0.0023 of their size against 0.0017).
         uint32_t pf[kSlabs][4];
 #pragma unroll
         for (int i = 0; i < kSlabs * 2; ++i) {

@@ -83,6 +83,9 @@ __device__ __forceinline__ int tiles_of(const Sched &s, const SeqInfo &q) {
   return (q.q + s.tile_tokens - 1) / s.tile_tokens;
 }
 
+// One thread adds a sequence's tiles up, and resolve walks them again: 0.1 us a tile. Nothing next to the work of a prompt with
+// keys, but all there is to a call of very many empty tiles (32768 new tokens of 64 query heads to a key head and no keys, 8192
+// tiles: 904 us as one sequence, 97 as 128).
 __device__ __forceinline__ long long head_cost(const Sched &s, const SeqInfo &q) {
   long long c = 0;
   for (int t = 0, i = 0; t < q.q; t += s.tile_tokens, ++i) c += tile_info(s, q, i).n + s.tile_cost;

@@ -18,7 +18,7 @@
 //
 // What it takes: 2.2 us a block of 128 keys for 256 rows at D = 128, 1.9 us at D = 64 (the softmax warps issue in 43 % of
 // their cycles, two to a scheduler, and the exponentials take half of theirs), 2.5 to 3 us from a tile to the next, 5 us to
-// share the work out. A chunk of 2048 tokens over 32768, 32 + 8 heads of 128: 0.98 ms alone, 1.09 PFLOP/s (1.09 ms under the
+// share the work out (few dozen tiles a sequence; see head_cost for many more). A chunk of 2048 tokens over 32768, 32 + 8 heads of 128: 0.98 ms alone, 1.09 PFLOP/s (1.09 ms under the
 // power cap). Computing a part of the exponentials by a polynomial on the FMA pipe made it slower (1 of 8: +2 %, 3 of 8:
 // +10 %): instructions, not the special-function unit, are what these warps are short of.
 #pragma once
@@ -532,6 +532,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             tmem_st_wait();
           }
         }
+        // P goes to shared memory rounded to the cache's type, the sum takes the unrounded values (see the row kernel)
         const float sum = txa::row_block_exp_store<false, kElt>(s, p.qk_scale, -ref, 0, 0, p_row, row_xor);
         l_i = l_i * alpha + sum;
         m_i = m_next;

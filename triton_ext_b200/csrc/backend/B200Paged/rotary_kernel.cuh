@@ -3,7 +3,8 @@
 // Pair i of a head is the complex number x1 + i x2; a position p turns it by the angle 2 pi p f_i, where f_i is kept as
 // a 64-bit fraction of a turn. p * f_i in 64-bit wrap-around arithmetic IS the angle modulo whole turns, so no range
 // reduction loses anything at far positions (a product in fp32 is off by 0.06 rad at position 2^20 already); its upper
-// 32 bits go through sincospi.
+// 32 bits go through sincospi. What is left is f_i's own rounding, p 2^-65 of a turn: less than the cut to 32 bits up to
+// position 2^32, 2^-25 of a turn at 2^40.
 //
 // The work is one read and one write of every value: HBM bound when there are many tokens, launch bound when there are
 // few. A warp takes one token (a slice of its heads when there are few tokens): its lanes are the vectors of a head, by as

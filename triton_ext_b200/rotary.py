@@ -2,7 +2,8 @@
 `attention.attention`, with the gradient (the same turn backwards).
 
 `Rope` describes the rotation: how many columns of a head turn, how they pair up, and the angle a pair turns by per
-position. Angles are kept as 64-bit fractions of a whole turn, so position 2^31 is as exact as position 1.
+position. Angles are kept as 64-bit fractions of a whole turn, so position 2^31 is as exact as position 1 (2^40: to 2^-25 of a
+turn; each doubling from there loses a bit).
 
 torch is used for device memory, streams and autograd only. There is no fallback: if the shared library is missing or no
 B200 is present the calls raise.
