@@ -354,3 +354,17 @@ def test_outputs_that_overlap_themselves_are_refused(P):
                 call()
     assert bool((memory == 7.0).all())
     P.check()
+
+
+def test_a_list_that_reaches_into_the_lengths(P):
+    """The lengths may be a part of the caller's vector, and a list begin before them in it."""
+    n = 2000
+    memory = torch.zeros(1 + 3 * n, dtype=i32, device="cuda")
+    pools = [torch.zeros(1, 3 * n, 16, 1, 16, dtype=bf16, device="cuda") for _ in range(2)]
+    cache = P.PagedCache(*pools, torch.full((3 * n, 4), -1, dtype=i32, device="cuda"), memory[1:], torch.zeros(3 * n, dtype=i32, device="cuda"))
+    every = torch.arange(3 * n, dtype=i32, device="cuda")
+    cache.reserve(every[n:2 * n], torch.full((n,), 16, dtype=i32, device="cuda"))
+    cache.reserve(every[2 * n:], torch.full((n,), 16, dtype=i32, device="cuda"))
+    cache.truncate(every[n - 1:], memory[:2 * n + 1])              # row n - 1 + i to memory[i], which is row i - 1's length
+    P.check()
+    assert cache.lens.tolist() == [0] * (2 * n) + [16] * n

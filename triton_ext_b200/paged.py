@@ -284,7 +284,8 @@ class PagedCache:
             _invalid(f"{name} must be an int32 vector{f' of {n}' if n is not None else ''} on the device of the cache")
         # a part of the state (lengths as counts, say) would change under the kernel that reads it
         at, (t0, t1, l0, l1, r0, r1) = x.data_ptr(), self._own
-        if not x.is_contiguous() or l0 <= at < l1 or t0 <= at < t1 or r0 <= at < r1:
+        end = at + 4 * shape[0]
+        if not x.is_contiguous() or l0 < end and at < l1 or t0 < end and at < t1 or r0 < end and at < r1:
             return x.clone(memory_format=torch.contiguous_format)
         return x
 
